@@ -65,13 +65,17 @@ extern "C" {
  * counts the additions (fdk_abi_revision() is the library's).  A caller built against revision 0 of version 8
  * runs unchanged against this library; a caller whose struct is LARGER than the library's is refused (FDK_EABI). */
 #define FDK_ABI_VERSION 8
-#define FDK_ABI_REVISION 2
+#define FDK_ABI_REVISION 3
 
 typedef enum fdk_dtype {
     FDK_BF16 = 0,
     FDK_FP16 = 1,
     FDK_FP8_E4M3 = 2, /* OCP e4m3fn, KV cache only */
-    FDK_FP32 = 3      /* partials / packed-rank buffers only */
+    FDK_FP32 = 3,     /* partials / packed-rank buffers only */
+    FDK_MXFP4 = 4     /* (revision 3) KV cache only: OCP microscaling rows of 4-bit values.  A row of D values is D/2 bytes of
+                         e2m1 codes (value 2i in the low four bits of byte i) and, in a tensor of its own, D/32 e8m0 bytes,
+                         one per block of 32 consecutive values: value = code * 2^(byte - 127), byte 255: NaN.  Strides of
+                         both are in bytes */
 } fdk_dtype;
 
 typedef enum fdk_status {
@@ -123,7 +127,7 @@ typedef struct fdk_decode_args {
     int32_t q_dtype; /* FDK_BF16 | FDK_FP16 */
 
     /* caches [num_pages, P, Hkv, D] (v_cache: Dv, see v_head_dim); strides of the page, token-in-page and head axes */
-    int32_t kv_dtype; /* q_dtype | FDK_FP8_E4M3 */
+    int32_t kv_dtype; /* q_dtype | FDK_FP8_E4M3 | FDK_MXFP4 (rows of D/2 bytes, strides in bytes) */
     const void* k_cache;
     const void* v_cache;
     int64_t k_stride_page, k_stride_tok, k_stride_head;
@@ -205,6 +209,15 @@ typedef struct fdk_decode_args {
      * follow v_head_dim: out is [B, Hq, Dv], the packed lse sits at out[b, h, Dv], fdk_workspace_bytes takes Dv. */
     int32_t v_head_dim;
     int32_t reserved3;
+
+    /* (revision 3) kv_dtype FDK_MXFP4: the scale bytes of the caches, [num_pages, P, Hkv, D/32], with byte strides of the
+     * page, token and head axes (any alignment).  k_scale / v_scale are not read.  Built for head_dim 64, 128 and 256 with
+     * v_head_dim = head_dim on the matrix-core path; no single-launch form; with counters, too, a forced split count runs as
+     * one workgroup per piece.  A value takes part as code * 2^(byte - 127) converted to q's dtype, exact within its range */
+    const uint8_t* k_block_scale;
+    const uint8_t* v_block_scale;
+    int64_t kbs_stride_page, kbs_stride_tok, kbs_stride_head;
+    int64_t vbs_stride_page, vbs_stride_tok, vbs_stride_head;
 } fdk_decode_args;
 
 #define FDK_FLAG_PACK_LSE 1u /* also store lse, converted to out_dtype, at out[b, h, D] (flash_decode.py:446-449) */
@@ -288,6 +301,26 @@ typedef struct fdk_kv_append_args {
     int64_t q_out_stride_b, q_out_stride_t, q_out_stride_h;
 } fdk_kv_append_args;
 
+/* (revision 3) Conversion between 16-bit rows and MXFP4 rows (see FDK_MXFP4): n0 x n1 x n2 rows of num_values values, each
+ * tensor with strides of its three row axes (elements; bytes for codes and scales), values contiguous.
+ *   fdk_mx_quantize    writes codes and scales: the scale of a block is the smallest power of two with amax <= 7 scales,
+ *                         within [2^-126, 2^125] for bf16 and [2^-126, 2^13] for fp16 (so that 6 scales are finite in the
+ *                         type); codes are rounded to nearest, ties to even, and saturate at 6.  A block that holds an
+ *                         infinity or a NaN gets scale byte 255
+ *   fdk_mx_dequantize  writes x: code * 2^(byte - 127) in x_dtype */
+typedef struct fdk_mxfp4_args {
+    uint32_t struct_size;
+    uint32_t flags;       /* FDK_FLAG_DRY_RUN */
+    void* x;              /* FDK_BF16 | FDK_FP16, 16-byte aligned rows */
+    uint8_t* codes;       /* 4-byte aligned rows of num_values / 2 bytes */
+    uint8_t* scales;      /* rows of num_values / 32 bytes */
+    int64_t x_stride[3], codes_stride[3], scales_stride[3];
+    int32_t n[3];
+    int32_t num_values;   /* a positive multiple of 32 */
+    int32_t x_dtype;
+    int32_t reserved;
+} fdk_mxfp4_args;
+
 struct fdk_measure_args; /* include/fdk_measure.h */
 
 int fdk_abi_version(void);
@@ -346,6 +379,10 @@ int fdk_combine(const fdk_decode_args* args, void* hip_stream);
 
 /* Merge R per-rank local results into the global attention output. */
 int fdk_combine_ranks(const fdk_combine_ranks_args* args, void* hip_stream);
+
+/* 16-bit rows to MXFP4 rows and back (see fdk_mxfp4_args). */
+int fdk_mx_quantize(const fdk_mxfp4_args* args, void* hip_stream);
+int fdk_mx_dequantize(const fdk_mxfp4_args* args, void* hip_stream);
 
 /* Normalise, rotate and append the new tokens (see fdk_kv_append_args). */
 int fdk_kv_append(const fdk_kv_append_args* args, void* hip_stream);

@@ -1,0 +1,204 @@
+"""MXFP4 caches on the GPU: the conversions against the format's definition, the decode against attention in 64 bits over
+the values that the codes stand for."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from oracle import mxfp4
+from tests.mxfp4_cases import decode_tolerances, make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+def _close(got, want, tol):
+    """|got - want| <= tol, infinities and NaN in the same places."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    same = (got == want) | torch.isnan(want)
+    off = torch.where(same, torch.zeros_like(want), (got - want).abs())
+    worst = float((off - tol).max())
+    assert worst <= 0, f"off by {float(off.max()):.3g}, {worst:.3g} over the tolerance"
+
+
+def _run(lens, hq, hkv, d, page, dtype, seed, layout="token", soft_cap=0.0, cuda_device=None, **kw):
+    import triton_distributed_amd as tda
+    (kc, ks, k64, vc, vs, v64), table = make_cache(lens, page, hkv, d, dtype, seed, layout)
+    g = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn(len(lens), hq, d, generator=g).to(dtype)
+    sm_scale = d ** -0.5
+    dev = lambda t: t.to(cuda_device)
+    # (.to keeps the strides of the "head" layout)
+    out, lse = tda.flash_decode(dev(q), dev(kc), dev(vc), dev(table), torch.tensor(lens, dtype=torch.int32, device=cuda_device),
+                                sm_scale, soft_cap=soft_cap, k_scale=dev(ks), v_scale=dev(vs), **kw)
+    torch.cuda.synchronize()
+    o64, l64, spread = mxfp4.decode(q, k64, v64, table, lens, sm_scale, soft_cap)
+    tol_o, tol_l = decode_tolerances(q, k64, spread, o64, l64, sm_scale, dtype)
+    _close(out, o64, tol_o)
+    _close(lse, l64, tol_l)
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_code_and_scale_dequantizes_exactly(cuda_device, dtype):
+    import triton_distributed_amd as tda
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 16, 16).expand(256, 16, 16).contiguous()
+    scales = torch.arange(256, dtype=torch.uint8).view(256, 1, 1).expand(256, 16, 1).contiguous()
+    got = tda.mxfp4_dequantize(codes.to(cuda_device), scales.to(cuda_device), dtype).cpu()
+    want = mxfp4.dequantize(codes, scales).to(dtype)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantize_matches_the_definition(cuda_device, dtype):
+    """Random rows over the whole range of exponents, every 16-bit pattern, zeros, infinities and NaN."""
+    import triton_distributed_amd as tda
+    g = torch.Generator().manual_seed(5)
+    lo, hi = (-130, 128) if dtype == torch.bfloat16 else (-24, 16)
+    x = torch.randn(3000, 64, generator=g).double() * 2.0 ** torch.randint(lo, hi, (3000, 1), generator=g).double()
+    top = torch.finfo(dtype).max
+    x = x.clamp(-top, top).to(dtype)
+    every = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype).view(1024, 64)
+    zeros = torch.zeros(2, 64, dtype=dtype)
+    zeros[1] = -0.0
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, -0.25, -5.0, 1.0] + [0.0] * 52, dtype=dtype)
+    x = torch.cat((x, every, zeros, ties[None], ties[None] * 2.0 ** 8))
+    codes, scales = tda.mxfp4_quantize(x.to(cuda_device))
+    want_c, want_s = mxfp4.quantize(x)
+    assert torch.equal(scales.cpu(), want_s)
+    fine = (want_s != 255).repeat_interleave(16, -1)
+    assert torch.equal(codes.cpu()[fine], want_c[fine])
+    back = tda.mxfp4_dequantize(codes, scales, dtype).cpu()
+    assert torch.isfinite(back[(want_s != 255).repeat_interleave(32, -1)]).all()
+    assert back[(want_s == 255).repeat_interleave(32, -1)].isnan().all()
+
+
+def test_conversions_of_strided_rows(cuda_device):
+    """Rows of a cache laid out by heads, a slice of wider rows; what lies between them stays."""
+    import triton_distributed_amd as tda
+    x = torch.randn(5, 3, 7, 192, device=cuda_device, dtype=torch.bfloat16)[..., 64:160]
+    codes = torch.full((5, 7, 3, 64), 99, dtype=torch.uint8, device=cuda_device)
+    view = codes.transpose(1, 2)[..., 4:52]
+    scales = torch.full((5, 3, 7, 5), 98, dtype=torch.uint8, device=cuda_device)
+    tda.mxfp4_quantize(x, view, scales[..., 1:4])
+    want_c, want_s = mxfp4.quantize(x.cpu())
+    assert torch.equal(view.cpu(), want_c) and torch.equal(scales[..., 1:4].cpu(), want_s)
+    assert (codes[..., :4] == 99).all() and (codes[..., 52:] == 99).all()
+    assert (scales[..., 0] == 98).all() and (scales[..., 4] == 98).all()
+    out = torch.zeros(5, 3, 7, 192, device=cuda_device, dtype=torch.float16)
+    tda.mxfp4_dequantize(view, scales[..., 1:4], out=out[..., 64:160])
+    assert torch.equal(out[..., 64:160].cpu(), mxfp4.dequantize(want_c, want_s).half())
+    assert (out[..., :64] == 0).all() and (out[..., 160:] == 0).all()
+    assert tda.mxfp4_quantize(x[:0])[0].shape == (0, 3, 7, 48)
+
+
+LENS = [0, 1, 15, 16, 17, 31, 32, 33, 255, 256, 257, 511, 700, 1029]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 5, 16, 48, 64])
+def test_lengths_pages_head_dims(cuda_device, dtype, d, page):
+    _run(LENS, 8, 2, d, page, dtype, 10 * d + page, cuda_device=cuda_device)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (6, 2), (16, 1), (17, 1), (40, 1), (96, 3), (64, 8), (20, 4)])
+@pytest.mark.parametrize("layout", ["token", "head"])
+def test_head_layouts(cuda_device, hq, hkv, layout):
+    _run([300, 0, 77, 1], hq, hkv, 128, 16, torch.bfloat16, 100 + hq, layout, cuda_device=cuda_device)
+
+
+@pytest.mark.parametrize("kv_split", [-1, 1, 7, 64])
+@pytest.mark.parametrize("page", [3, 16])
+def test_split_counts(cuda_device, kv_split, page):
+    _run([2000, 5, 0, 1111], 8, 2, 128, page, torch.bfloat16, 7, kv_split=kv_split, cuda_device=cuda_device)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [7, 32])
+def test_equal_shares(cuda_device, d, page):
+    """The plan that cuts the whole batch into equal shares, whatever the planner would choose."""
+    _run([3000, 1, 0, 64, 1700, 33, 0, 900], 10, 2, d, page, torch.bfloat16, 8, force_balanced=True, cuda_device=cuda_device)
+
+
+def test_soft_cap_and_known_lengths(cuda_device):
+    _run([600, 590, 600], 4, 1, 128, 16, torch.float16, 9, soft_cap=5.0, cuda_device=cuda_device)
+    _run([640] * 40, 32, 8, 128, 16, torch.bfloat16, 9, max_kv_len=640, min_kv_len=640, cuda_device=cuda_device)
+
+
+def test_one_dominant_token(cuda_device):
+    """Logits over a range of several hundred: the running maximum moves by more and by less than the step at which the
+    accumulators are rescaled."""
+    import triton_distributed_amd as tda
+    lens = [777]
+    (kc, ks, k64, vc, vs, v64), table = make_cache(lens, 16, 1, 128, torch.bfloat16, 4)
+    q = torch.randn(1, 4, 128, generator=torch.Generator().manual_seed(3)).bfloat16() * 8
+    out, lse = tda.flash_decode(q.to(cuda_device), kc.to(cuda_device), vc.to(cuda_device), table.to(cuda_device),
+                                torch.tensor(lens, dtype=torch.int32, device=cuda_device), 0.5, k_scale=ks.to(cuda_device),
+                                v_scale=vs.to(cuda_device))
+    o64, l64, spread = mxfp4.decode(q, k64, v64, table, lens, 0.5)
+    tol_o, tol_l = decode_tolerances(q, k64, spread, o64, l64, 0.5, torch.bfloat16)
+    _close(out, o64, tol_o)
+    _close(lse, l64, tol_l)
+
+
+def test_typed_caches_packed_result_static_scratch(cuda_device):
+    """float4 / e8m0 spelling of the types, the packed drop-in result and the entry that allocates nothing: same bits."""
+    import triton_distributed_amd as tda
+    from triton_distributed_amd import _lib
+    lens = [1500, 40, 0]
+    (kc, ks, k64, vc, vs, v64), table = make_cache(lens, 16, 2, 128, torch.bfloat16, 12)
+    dev = lambda t: t.to(cuda_device)
+    q = dev(torch.randn(3, 8, 128, generator=torch.Generator().manual_seed(3)).bfloat16())
+    kc, ks, vc, vs, table = dev(kc), dev(ks), dev(vc), dev(vs), dev(table)
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    out, lse = tda.flash_decode(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs)
+    f4, e8 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+    out2, lse2 = tda.flash_decode(q, kc.view(f4), vc.view(f4), table, n, 0.1, k_scale=ks.view(e8), v_scale=vs.view(e8))
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    call = tda.prepare_decode(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs, static_scratch=True)
+    assert call.plan.num_splits > 1
+    out3, lse3 = call.run_static()
+    assert torch.equal(out, out3) and torch.equal(lse, lse3)
+    packed = torch.empty(3, 8, 129, dtype=torch.bfloat16, device=cuda_device)
+    tda.prepare_decode(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs, packed_out=packed, want_lse=False).run()
+    assert torch.equal(packed[..., :128], out) and torch.equal(packed[..., 128], lse.bfloat16())
+    # counters are accepted (and left at zero): one workgroup per piece
+    call = tda.prepare_decode(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs, kv_split=20)
+    out4, lse4 = call.run()
+    torch.testing.assert_close(out4.float(), out.float(), atol=2e-2, rtol=2e-2)
+    rc = _lib.load().fdk_decode_splitkv(C.byref(call.args), torch.cuda.current_stream().cuda_stream)
+    rc2 = _lib.load().fdk_combine(C.byref(call.args), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and rc2 == 0
+    assert torch.equal(call.out, out4) and torch.equal(call.lse, lse4)
+
+
+def test_captured_and_replayed_on_another_stream(cuda_device):
+    """A captured call, replayed while eager calls of other shapes run in between, follows the lengths on the device."""
+    import triton_distributed_amd as tda
+    (kc, ks, k64, vc, vs, v64), table = make_cache([900, 900], 16, 2, 128, torch.bfloat16, 13)
+    dev = lambda t: t.to(cuda_device)
+    qc = torch.randn(2, 8, 128, generator=torch.Generator().manual_seed(3)).bfloat16()
+    q, kc, ks, vc, vs, tb = dev(qc), dev(kc), dev(ks), dev(vc), dev(vs), dev(table)
+    n = torch.tensor([5, 5], dtype=torch.int32, device=cuda_device)
+    call = tda.prepare_decode(q, kc, vc, tb, n, 0.1, k_scale=ks, v_scale=vs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call.run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            call.run()
+    for lens in ([900, 1], [0, 333], [512, 512]):
+        n.copy_(torch.tensor(lens, dtype=torch.int32))
+        tda.flash_decode(q, kc, vc, tb, n, 0.1, k_scale=ks, v_scale=vs, kv_split=9)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        o64, l64, spread = mxfp4.decode(qc, k64, v64, table, lens, 0.1)
+        tol_o, tol_l = decode_tolerances(qc, k64, spread, o64, l64, 0.1, torch.bfloat16)
+        _close(call.out, o64, tol_o)
+        _close(call.lse, l64, tol_l)
+        assert math.isfinite(float(call.out.float().sum()))

@@ -1,0 +1,156 @@
+"""MXFP4 caches, without a GPU: what the entry points refuse, how calls are planned, and the oracle itself."""
+import ctypes as C
+
+import pytest
+import torch
+
+from oracle import mxfp4
+from triton_distributed_amd import _lib
+from triton_distributed_amd._lib import FdkDecodeArgs, FdkMxfp4Args, FdkPlan
+import triton_distributed_amd as tda
+
+
+def _args(**kw):
+    """A valid dry-run argument block on fake (never dereferenced) pointers: B32 32q/8kv P16 N4096, 4-bit cache."""
+    a = FdkDecodeArgs()
+    a.struct_size = C.sizeof(FdkDecodeArgs)
+    a.flags = _lib.FDK_FLAG_DRY_RUN
+    a.q, a.k_cache, a.v_cache = 0x10000, 0x20000, 0x30000
+    a.block_table, a.kv_lens, a.out, a.lse = 0x40000, 0x50000, 0x60000, 0x70000
+    a.q_dtype = a.out_dtype = _lib.FDK_BF16
+    a.kv_dtype = _lib.FDK_MXFP4
+    a.batch, a.num_q_heads, a.num_kv_heads, a.head_dim = 32, 32, 8, 128
+    a.page_size, a.max_pages = 16, 256
+    a.q_stride_b, a.q_stride_h = 32 * 128, 128
+    a.k_stride_page, a.k_stride_tok, a.k_stride_head = 16 * 8 * 64, 8 * 64, 64
+    a.v_stride_page, a.v_stride_tok, a.v_stride_head = 16 * 8 * 64, 8 * 64, 64
+    a.k_block_scale, a.v_block_scale = 0x80001, 0x90003
+    a.kbs_stride_page, a.kbs_stride_tok, a.kbs_stride_head = 16 * 8 * 4, 8 * 4, 4
+    a.vbs_stride_page, a.vbs_stride_tok, a.vbs_stride_head = 16 * 8 * 4, 8 * 4, 4
+    a.table_stride_b = 256
+    a.sm_scale = 0.088
+    a.out_stride_b, a.out_stride_h, a.lse_stride_b = 32 * 128, 128, 32
+    a.max_kv_len = a.min_kv_len = 4096
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def _rc(a):
+    return _lib.load().fdk_decode(C.byref(a), None)
+
+
+def test_valid_calls_pass_a_dry_run():
+    assert _rc(_args()) == 0
+    assert _rc(_args(q_dtype=_lib.FDK_FP16)) == 0
+    for d in (64, 256):
+        a = _args(head_dim=d, k_stride_head=d // 2, v_stride_head=d // 2, k_stride_tok=4 * d, v_stride_tok=4 * d,
+                  k_stride_page=64 * d, v_stride_page=64 * d, kbs_stride_head=d // 32, vbs_stride_head=d // 32,
+                  q_stride_h=d, q_stride_b=32 * d, out_stride_h=d, out_stride_b=32 * d)
+        assert _rc(a) == 0, _lib.load().fdk_last_error()
+
+
+@pytest.mark.parametrize("field,value,code", [
+    ("k_block_scale", 0, _lib.FDK_ENULL), ("v_block_scale", 0, _lib.FDK_ENULL),
+    ("algo", _lib.FDK_ALGO_VALU, _lib.FDK_EUNSUPPORTED),
+    ("flags", _lib.FDK_FLAG_DRY_RUN | _lib.FDK_FLAG_SINGLE_LAUNCH, _lib.FDK_EUNSUPPORTED),
+    ("head_dim", 192, _lib.FDK_EUNSUPPORTED), ("v_head_dim", 64, _lib.FDK_EUNSUPPORTED),
+    ("q_dtype", _lib.FDK_MXFP4, _lib.FDK_EUNSUPPORTED), ("out_dtype", _lib.FDK_MXFP4, _lib.FDK_EUNSUPPORTED),
+    ("k_stride_head", 32, _lib.FDK_ESHAPE), ("k_stride_tok", 8 * 64 + 8, _lib.FDK_EALIGN),
+    ("kbs_stride_head", 3, _lib.FDK_ESHAPE), ("vbs_stride_tok", -1, _lib.FDK_ESHAPE),
+    ("kbs_stride_page", 1 << 32, _lib.FDK_ESHAPE), ("vbs_stride_tok", 1 << 62, _lib.FDK_ESHAPE),
+])
+def test_refusals(field, value, code):
+    assert _rc(_args(**{field: value})) == code
+
+
+def test_a_caller_of_the_previous_revision_is_asked_for_scales():
+    a = _args(struct_size=FdkDecodeArgs.k_block_scale.offset)
+    assert _rc(a) == _lib.FDK_ENULL
+    a.kv_dtype = _lib.FDK_BF16
+    for f in ("k_stride_head", "v_stride_head"):
+        setattr(a, f, 128)
+    assert _rc(a) == 0
+
+
+def test_plans():
+    """Every plan takes one kv head per workgroup; a batch that fills the compute units alone is a single pass, short ones
+    are cut into chunks, long ragged ones into equal shares."""
+    plan = FdkPlan()
+    lib = _lib.load()
+    assert lib.fdk_plan(C.byref(_args()), 0, C.byref(plan)) == 0
+    assert (plan.num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 1, 0)
+    for kw in (dict(batch=2), dict(batch=3, min_kv_len=0), dict(batch=40, min_kv_len=0, max_kv_len=0, max_pages=8192, table_stride_b=8192),
+               dict(batch=4, max_pages=16384, table_stride_b=16384, max_kv_len=0, min_kv_len=0)):
+        assert lib.fdk_plan(C.byref(_args(**kw)), 0, C.byref(plan)) == 0
+        assert plan.kv_heads_per_wg == 1 and plan.algo == _lib.FDK_ALGO_MFMA
+        assert plan.num_splits > 1
+        assert not plan.balanced or plan.workgroups % 8 == 0
+
+
+def _conv(**kw):
+    a = FdkMxfp4Args()
+    a.struct_size = C.sizeof(FdkMxfp4Args)
+    a.flags = _lib.FDK_FLAG_DRY_RUN
+    a.x, a.codes, a.scales = 0x10000, 0x20000, 0x30001
+    a.x_stride, a.codes_stride, a.scales_stride = (C.c_int64 * 3)(0, 0, 128), (C.c_int64 * 3)(0, 0, 64), (C.c_int64 * 3)(0, 0, 4)
+    a.n = (C.c_int32 * 3)(1, 1, 1000)
+    a.num_values, a.x_dtype = 128, _lib.FDK_BF16
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), (dict(num_values=100), _lib.FDK_ESHAPE), (dict(num_values=0), _lib.FDK_ESHAPE), (dict(x_dtype=_lib.FDK_FP32), _lib.FDK_EUNSUPPORTED),
+    (dict(x=0), _lib.FDK_ENULL), (dict(x=0x10008), _lib.FDK_EALIGN), (dict(codes=0x20002), _lib.FDK_EALIGN),
+    (dict(x_stride=(C.c_int64 * 3)(0, 0, 132)), _lib.FDK_EALIGN), (dict(codes_stride=(C.c_int64 * 3)(0, 0, 66)), _lib.FDK_EALIGN),
+    (dict(n=(C.c_int32 * 3)(1, -1, 1)), _lib.FDK_ESHAPE), (dict(n=(C.c_int32 * 3)(0, 1, 1), x=0), 0),
+    (dict(n=(C.c_int32 * 3)(2 ** 31 - 1, 2 ** 31 - 1, 4)), _lib.FDK_ESHAPE), (dict(struct_size=8), _lib.FDK_EABI),
+])
+def test_conversion_refusals(kw, code):
+    lib = _lib.load()
+    for fn in (lib.fdk_mx_quantize, lib.fdk_mx_dequantize):
+        assert fn(C.byref(_conv(**kw)), None) == code
+
+
+def test_python_refusals():
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="live on the GPU"):
+        tda.mxfp4_quantize(x)
+    with pytest.raises(ValueError, match="bf16 / fp16"):
+        tda.mxfp4_quantize(x.float())
+    with pytest.raises(ValueError, match="multiple of 32"):
+        tda.mxfp4_quantize(x[:, :48])
+    with pytest.raises(ValueError, match="codes"):
+        tda.mxfp4_quantize(x, torch.zeros(4, 32, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="scales"):
+        tda.mxfp4_dequantize(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 3, dtype=torch.uint8))
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    cache, scale = torch.zeros(2, 16, 2, 64, dtype=torch.uint8), torch.zeros(2, 16, 2, 4, dtype=torch.uint8)
+    table, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="live on the GPU"):
+        tda.flash_decode(q, cache, cache, table, n, 0.1, k_scale=scale, v_scale=scale)
+    plan = tda.get_split_kv_plan(q, cache, cache, table, n, num_cus=256)
+    assert plan.algo == "mfma"
+    from triton_distributed_amd.flash_decode import _check_block_scales
+    for bad in (None, scale[..., :3], scale.float(), scale[:1], scale.transpose(1, 3)):
+        with pytest.raises(ValueError, match="k_scale"):
+            _check_block_scales("k_scale", bad, cache)
+
+
+def test_oracle_by_hand():
+    """Codes and scales worked out by hand."""
+    x = torch.zeros(1, 64, dtype=torch.bfloat16)
+    x[0, :6] = torch.tensor([7.0, -6.5, 0.25, 0.75, 2.5, -1.0])              # amax 7: scale 1
+    x[0, 32:36] = torch.tensor([7.0625, 1.0, -14.0, 5.0])                    # amax 14: scale 2
+    codes, scales = mxfp4.quantize(x)
+    assert scales.tolist() == [[127, 128]]
+    assert codes[0, :3].tolist() == [7 | (15 << 4), 0 | (2 << 4), 4 | (10 << 4)]
+    assert codes[0, 16:18].tolist() == [6 | (1 << 4), 15 | (4 << 4)]
+    v = mxfp4.dequantize(codes, scales)
+    assert v[0, :6].tolist() == [6.0, -6.0, 0.0, 1.0, 2.0, -1.0] and v[0, 32:36].tolist() == [8.0, 1.0, -12.0, 4.0]
+    x[0, 3] = float("inf")
+    assert mxfp4.quantize(x)[1].tolist() == [[255, 128]]
+    assert mxfp4.quantize(torch.full((1, 32), 65504.0, dtype=torch.float16))[1].tolist() == [[127 + 13]]
+    assert mxfp4.quantize(torch.zeros(1, 32, dtype=torch.float16))[1].tolist() == [[1]]

@@ -12,10 +12,10 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libfdk.so"
 
 FDK_ABI_VERSION = 8
-FDK_ABI_REVISION = 2      # the library may be newer (its structs only grow at the end), never older
+FDK_ABI_REVISION = 3      # the library may be newer (its structs only grow at the end), never older
 
 # fdk_dtype
-FDK_BF16, FDK_FP16, FDK_FP8_E4M3, FDK_FP32 = 0, 1, 2, 3
+FDK_BF16, FDK_FP16, FDK_FP8_E4M3, FDK_FP32, FDK_MXFP4 = 0, 1, 2, 3, 4
 # fdk_status
 FDK_OK, FDK_ENULL, FDK_EALIGN, FDK_ESHAPE, FDK_EUNSUPPORTED, FDK_EWORKSPACE, FDK_EABI = 0, -1, -2, -3, -4, -5, -6
 # fdk_algo
@@ -28,7 +28,7 @@ FDK_STATIC_SCRATCH_BYTES = 32 << 20
 EXPORTS = (
     "fdk_abi_version", "fdk_abi_revision", "fdk_last_error", "fdk_device_cus", "fdk_plan", "fdk_workspace_bytes",
     "fdk_decode", "fdk_decode_splitkv", "fdk_combine", "fdk_combine_ranks", "fdk_counters_len", "fdk_kv_append",
-    "fdk_decode_static", "fdk_length_feedback_alloc", "fdk_length_feedback_free",
+    "fdk_decode_static", "fdk_length_feedback_alloc", "fdk_length_feedback_free", "fdk_mx_quantize", "fdk_mx_dequantize",
 )
 # declared in include/fdk_measure.h
 MEASURE_EXPORTS = ("fdk_probe_linear_read",)
@@ -63,6 +63,9 @@ class FdkDecodeArgs(C.Structure):
         ("reserved1", C.c_void_p), ("reserved2", C.c_int64),
         ("measure", C.c_void_p),           # FdkMeasureArgs*, null in product use
         ("v_head_dim", C.c_int32), ("reserved3", C.c_int32),     # (revision 2) 0: V rows as long as q / K rows
+        ("k_block_scale", C.c_void_p), ("v_block_scale", C.c_void_p),      # (revision 3) FDK_MXFP4 caches
+        ("kbs_stride_page", C.c_int64), ("kbs_stride_tok", C.c_int64), ("kbs_stride_head", C.c_int64),
+        ("vbs_stride_page", C.c_int64), ("vbs_stride_tok", C.c_int64), ("vbs_stride_head", C.c_int64),
     ]
 
 
@@ -107,6 +110,15 @@ class FdkKvAppendArgs(C.Structure):
         ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
         ("q_out", C.c_void_p), ("q_out_stride_b", C.c_int64), ("q_out_stride_t", C.c_int64),
         ("q_out_stride_h", C.c_int64),
+    ]
+
+
+class FdkMxfp4Args(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("flags", C.c_uint32),
+        ("x", C.c_void_p), ("codes", C.c_void_p), ("scales", C.c_void_p),
+        ("x_stride", C.c_int64 * 3), ("codes_stride", C.c_int64 * 3), ("scales_stride", C.c_int64 * 3),
+        ("n", C.c_int32 * 3), ("num_values", C.c_int32), ("x_dtype", C.c_int32), ("reserved", C.c_int32),
     ]
 
 
@@ -162,6 +174,10 @@ def load() -> C.CDLL:
     lib.fdk_length_feedback_free.argtypes = [C.c_void_p]
     lib.fdk_kv_append.restype = C.c_int
     lib.fdk_kv_append.argtypes = [C.POINTER(FdkKvAppendArgs), C.c_void_p]
+    for name in ("fdk_mx_quantize", "fdk_mx_dequantize"):
+        fn = getattr(lib, name)
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(FdkMxfp4Args), C.c_void_p]
     if lib.fdk_abi_version() != FDK_ABI_VERSION or lib.fdk_abi_revision() < FDK_ABI_REVISION:
         raise ImportError(f"{path}: ABI {lib.fdk_abi_version()}.{lib.fdk_abi_revision()}, this package needs "
                           f"{FDK_ABI_VERSION}.{FDK_ABI_REVISION} or a later revision")

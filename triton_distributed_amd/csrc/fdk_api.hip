@@ -11,6 +11,7 @@
 
 #include "../../include/fdk_measure.h"
 #include "fdk_device.h"
+#include "fdk_mxfp4.h"
 
 namespace {
 
@@ -30,11 +31,15 @@ int elem_size(int dt) {
     switch (dt) {
         case FDK_BF16:
         case FDK_FP16: return 2;
-        case FDK_FP8_E4M3: return 1;
+        case FDK_FP8_E4M3:
+        case FDK_MXFP4: return 1;       // (strides of 4-bit rows are in bytes)
         case FDK_FP32: return 4;
         default: return 0;
     }
 }
+
+// bytes that `values` cached values take, with their block scales
+double kv_bytes(int dt, double values) { return dt == FDK_MXFP4 ? values * (0.5 + 1.0 / fdk::kMxBlock) : values * elem_size(dt); }
 
 int ilog2_exact(int x) {
     if (x <= 0 || (x & (x - 1)) != 0) return -1;
@@ -157,6 +162,15 @@ inline bool plain_dims(int dk, int dv) { return dk == dv && (dk == 64 || dk == 1
 // 16-bit caches
 inline bool two_segment_dims(int dk, int dv) { return (dk == 192 && (dv == 192 || dv == 128)) || (dk == 576 && dv == 512); }
 
+// byte strides of an MXFP4 cache's scales (page, token, head)
+int check_scale_strides(int64_t sp, int64_t st, int64_t sh, int head_dim, int num_kv_heads, int page_size) {
+    if (sp < 0 || st < 0 || sh < 0) return fail(FDK_ESHAPE, "negative block scale stride");
+    if (num_kv_heads > 1 && sh < head_dim / fdk::kMxBlock) return fail(FDK_ESHAPE, "block scale head stride < head_dim / 32");
+    if (sp >= ((int64_t)1 << 32) || st >= ((int64_t)1 << 28) || page_size * st >= ((int64_t)1 << 32))
+        return fail(FDK_ESHAPE, "block scale strides too large: a page must span less than 4 GiB");
+    return FDK_OK;
+}
+
 // (a: a block in this library's layout, from adopt_call)
 int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) {
     if (a->batch < 0) return fail(FDK_ESHAPE, "batch %d < 0", a->batch);
@@ -188,8 +202,14 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
         return fail(FDK_ESHAPE, "num_splits %d outside [0, %d]", a->num_splits, kMaxSplits);
     if (a->q_dtype != FDK_BF16 && a->q_dtype != FDK_FP16)
         return fail(FDK_EUNSUPPORTED, "q_dtype %d (bf16 or fp16 only)", a->q_dtype);
-    if (a->kv_dtype != a->q_dtype && a->kv_dtype != FDK_FP8_E4M3)
-        return fail(FDK_EUNSUPPORTED, "kv_dtype %d must equal q_dtype or be fp8_e4m3", a->kv_dtype);
+    if (a->kv_dtype != a->q_dtype && a->kv_dtype != FDK_FP8_E4M3 && a->kv_dtype != FDK_MXFP4)
+        return fail(FDK_EUNSUPPORTED, "kv_dtype %d must equal q_dtype or be fp8_e4m3 or mxfp4", a->kv_dtype);
+    if (a->kv_dtype == FDK_MXFP4) {
+        if (!plain_dims(a->head_dim, dv))
+            return fail(FDK_EUNSUPPORTED, "head_dim %d / v_head_dim %d: not built for mxfp4 caches (64, 128, 256)", a->head_dim, dv);
+        if (a->algo == FDK_ALGO_VALU) return fail(FDK_EUNSUPPORTED, "mxfp4 caches: built on the matrix-core path");
+        if (a->flags & FDK_FLAG_SINGLE_LAUNCH) return fail(FDK_EUNSUPPORTED, "mxfp4 caches: the single-launch form is not built");
+    }
     if (a->algo < FDK_ALGO_AUTO || a->algo > FDK_ALGO_MFMA) return fail(FDK_EUNSUPPORTED, "algo %d", a->algo);
     if (a->length_feedback && (reinterpret_cast<uintptr_t>(a->length_feedback) & 15u))
         return fail(FDK_EALIGN, "length_feedback must be 16-byte aligned");
@@ -235,9 +255,18 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
     if (a->kv_dtype == FDK_FP8_E4M3 &&
         ((reinterpret_cast<uintptr_t>(a->k_scale) & 3u) || (reinterpret_cast<uintptr_t>(a->v_scale) & 3u)))
         return fail(FDK_EALIGN, "k_scale / v_scale must be 4-byte aligned");
-    if ((a->k_stride_head < a->head_dim || a->v_stride_head < dv) && a->num_kv_heads > 1)
+    const int per = a->kv_dtype == FDK_MXFP4 ? 2 : 1;               // values per element of a cache row
+    if ((a->k_stride_head < a->head_dim / per || a->v_stride_head < dv / per) && a->num_kv_heads > 1)
         return fail(FDK_ESHAPE, "cache head stride < head_dim (k %lld, v %lld)", (long long)a->k_stride_head,
                     (long long)a->v_stride_head);
+    if (a->kv_dtype == FDK_MXFP4 && (need_out || need_workspace_only)) {        // (a plan alone needs no scales)
+        if (!a->k_block_scale || !a->v_block_scale)
+            return fail(FDK_ENULL, "k_block_scale / v_block_scale are required for an mxfp4 cache");
+        const int64_t bs[2][3] = {{a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head},
+                                  {a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head}};
+        for (const auto& b : bs)
+            if (int rc = check_scale_strides(b[0], b[1], b[2], a->head_dim, a->num_kv_heads, a->page_size)) return rc;
+    }
     if (a->table_stride_b < a->max_pages)
         return fail(FDK_ESHAPE, "table_stride_b %lld < max_pages %d", (long long)a->table_stride_b, a->max_pages);
 
@@ -253,7 +282,6 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
         if (a->lse && a->lse_stride_b < a->num_q_heads)
             return fail(FDK_ESHAPE, "lse_stride_b %lld < Hq", (long long)a->lse_stride_b);
     }
-    (void)need_workspace_only;
     return FDK_OK;
 }
 
@@ -306,9 +334,8 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
     const bool alike = a->min_kv_len > 0 && (int64_t)a->min_kv_len * 32 >= max_len * 31;
     // what streaming the batch's cache takes (the shared-tile kernels are bound by the 16-bit tile they stage, not by
     // the bytes they read: a one-byte cache takes them as long as a 16-bit one, and is planned like one)
-    const int stream_elem = tile_heads > 16 ? 2 : elem_size(a->kv_dtype);
-    const double stream_us = (double)batch * (double)max_len * a->num_kv_heads * (double)(a->head_dim + v_dim(a)) *
-                             stream_elem / kStreamBytesPerUs;
+    const double stream_us = (double)batch * (double)max_len * a->num_kv_heads *
+                             kv_bytes(tile_heads > 16 ? FDK_BF16 : a->kv_dtype, (double)(a->head_dim + v_dim(a))) / kStreamBytesPerUs;
     bool rebalance = false;
     // (measurement aid: equal shares wherever they can run, to time them against the plan chosen here)
     const bool force_balanced = a->measure && a->measure->force_balanced && algo == FDK_ALGO_MFMA && a->num_splits <= 0 &&
@@ -325,7 +352,7 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
         }
         if (rebalance) {
             kv_heads_per_wg = a->num_kv_heads % 2 ? 1 : 2;
-            if (tile_heads > 16) kv_heads_per_wg = 1;
+            if (tile_heads > 16 || a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = 1;
             units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
         }
     }
@@ -432,7 +459,7 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
 // one and eight kv heads: 0 / 48 / 96 / 144 / 192 KB give 90.7 / 88.3 / 88.3 / 87.4 / 88.9, 165.7 / 164.0 / 162.3 /
 // 162.5 / 163.6 and 30.8 / 30.4 / 28.8 / 28.3 / 28.4 us per call).
 int piece_cost_granules(const fdk_decode_args* a, int kv_heads_per_wg) {
-    const int64_t granule_bytes = (int64_t)fdk::kBalanceGranule * kv_heads_per_wg * (a->head_dim + v_dim(a)) * elem_size(a->kv_dtype);
+    const int64_t granule_bytes = (int64_t)kv_bytes(a->kv_dtype, (double)fdk::kBalanceGranule * kv_heads_per_wg * (a->head_dim + v_dim(a)));
     // an even number: the kernel puts half of it in front of a sequence's tokens and half behind
     const int64_t c = 2 * ((kPieceOverheadBytes + granule_bytes) / (2 * granule_bytes));
     return (int)(c > 64 ? 64 : c);
@@ -549,6 +576,13 @@ int resolve(const fdk_decode_args* a, bool direct_ok, int num_cus, Resolved* r) 
 }
 
 int launch_split(const fdk_decode_args* a, const Resolved& r, hipStream_t stream) {
+    if (a->kv_dtype == FDK_MXFP4) {
+        const fdk::Mx4Scales scales{a->k_block_scale,   a->v_block_scale,   a->kbs_stride_page, a->kbs_stride_tok,
+                                    a->kbs_stride_head, a->vbs_stride_page, a->vbs_stride_tok,  a->vbs_stride_head};
+        const int rc = fdk::launch_splitkv_mx4(r.sp, scales, a->q_dtype, stream);
+        if (rc) return fail(rc, "split kernel launch failed: %s", hipGetErrorString((hipError_t)rc));
+        return FDK_OK;
+    }
     int rc = r.plan.algo == FDK_ALGO_MFMA ? fdk::launch_splitkv_mfma(r.sp, a->q_dtype, a->kv_dtype, stream)
                                           : fdk::launch_splitkv_valu(r.sp, a->q_dtype, a->kv_dtype, stream);
     if (rc) return fail(rc, "split kernel launch failed: %s", hipGetErrorString((hipError_t)rc));
@@ -797,6 +831,36 @@ int fdk_probe_linear_read(const void* buf, size_t bytes, int nontemporal, int wo
     if (rc) return fail(rc, "linear read launch failed: %s", hipGetErrorString((hipError_t)rc));
     return FDK_OK;
 }
+
+static int mxfp4_convert(const fdk_mxfp4_args* caller_args, bool quantize, void* hip_stream) {
+    g_err[0] = 0;
+    if (!caller_args) return fail(FDK_ENULL, "args is null");
+    fdk_mxfp4_args local;
+    if (int rc = adopt(caller_args, caller_args->struct_size, sizeof(fdk_mxfp4_args), "fdk_mxfp4_args", &local)) return rc;
+    const fdk_mxfp4_args* a = &local;
+    if (a->n[0] < 0 || a->n[1] < 0 || a->n[2] < 0) return fail(FDK_ESHAPE, "negative row count");
+    if (a->num_values <= 0 || a->num_values % fdk::kMxBlock) return fail(FDK_ESHAPE, "num_values %d: a positive multiple of 32", a->num_values);
+    if (a->x_dtype != FDK_BF16 && a->x_dtype != FDK_FP16) return fail(FDK_EUNSUPPORTED, "x_dtype %d (bf16 or fp16 only)", a->x_dtype);
+    if (!a->n[0] || !a->n[1] || !a->n[2]) return FDK_OK;
+    if ((unsigned __int128)a->n[0] * a->n[1] * a->n[2] * (a->num_values / 8) > (unsigned __int128)INT32_MAX * 256)
+        return fail(FDK_ESHAPE, "too many rows");
+    if (!a->x || !a->codes || !a->scales) return fail(FDK_ENULL, "x / codes / scales must be non-null");
+    for (int i = 0; i < 3; ++i) {
+        if (a->x_stride[i] < 0 || a->codes_stride[i] < 0 || a->scales_stride[i] < 0) return fail(FDK_ESHAPE, "negative stride");
+        if (a->n[i] > 1 && (a->x_stride[i] % 8 || a->codes_stride[i] % 4))
+            return fail(FDK_EALIGN, "rows of x must be 16-byte aligned, rows of codes 4-byte aligned");
+    }
+    if (!aligned16(a->x) || (reinterpret_cast<uintptr_t>(a->codes) & 3u))
+        return fail(FDK_EALIGN, "x must be 16-byte aligned, codes 4-byte aligned");
+    if (a->flags & FDK_FLAG_DRY_RUN) return FDK_OK;
+    const int rc = fdk::launch_mxfp4(*a, quantize, reinterpret_cast<hipStream_t>(hip_stream));
+    if (rc) return fail(rc, "mxfp4 conversion launch failed: %s", hipGetErrorString((hipError_t)rc));
+    return FDK_OK;
+}
+
+int fdk_mx_quantize(const fdk_mxfp4_args* args, void* hip_stream) { return mxfp4_convert(args, true, hip_stream); }
+
+int fdk_mx_dequantize(const fdk_mxfp4_args* args, void* hip_stream) { return mxfp4_convert(args, false, hip_stream); }
 
 int fdk_kv_append(const fdk_kv_append_args* caller_args, void* hip_stream) {
     g_err[0] = 0;

@@ -1,0 +1,448 @@
+// Split-KV paged GQA decode over an MXFP4 cache, matrix-core path, gfx950.
+//
+// The same contract, pieces, work distribution and partial rows as fdk_splitkv_mfma.h, for a cache of 4-bit rows (counterpart
+// in the reference: kernel_gqa_fwd_batch_decode_split_kv, python/triton_dist/kernels/nvidia/flash_decode.py:129-239, which
+// knows 16-bit caches only).  A workgroup works on one kv head and a tile of 16 q heads; its wavefronts interleave steps
+// of 32 tokens and are merged through LDS at the end of the piece.
+//
+// A row of 128 values is 64 bytes, so nothing goes through LDS on the way: K and V are loaded in the layout of the MFMA
+// operands, and converted in registers.
+//   K   lane (c, a) loads the a-th quarter of token c's row.  The k index of an MFMA is only a summation index: step ks of
+//       S^T = K Q^T multiplies values (D/4) a + 8 ks .. + 7, and Q^T is held in the same order.  A quarter row of 128
+//       values is one block of 32: one scale per lane and tile, applied by the conversion.
+//   V   lane (c, a) loads values (D/16) c .. + D/16 - 1 of the tokens whose probabilities the lane group a holds, converts
+//       them (again with the scale of its own block) and pairs the tokens up with byte permutes: operand A of
+//       O^T += V^T P^T, row m = c of column block db being value (D/16) c + db.
+//   P   straight from the softmax registers: lane (h, a) holds the logits of head h for tokens a, a + 4, a + 8, a + 12 of both
+//       halves of the step (K rows are assigned to the rows of S^T that way, so that one V load instruction reads four
+//       consecutive tokens).
+// The 64-byte rows of two kv heads share a 128-byte line, and so do the scales of four tokens and all heads: every unit of a
+// (sequence, split) runs on one XCD, with loads that leave the lines in its L2 (tiles_on_one_xcd).
+#pragma once
+
+#include "fdk_mxfp4.h"
+#include "fdk_splitkv_mfma.h"
+
+namespace fdk {
+
+namespace {
+
+constexpr int kStep = 32;                  // tokens per wavefront and step: two tiles of 16 rows, one k-step of P V
+
+template <int D>
+struct Mx4Tile {                           // one step in registers, as loaded
+    static constexpr int KW = D / 32;      // dwords of a quarter K row
+    static constexpr int VW = D >= 128 ? D / 128 : 1;     // dwords of a sixteenth of a V row (D = 64: half of one)
+    static constexpr int KS = D == 256 ? 2 : 1;           // blocks a quarter K row touches
+    uint32_t k[2][KW];
+    uint32_t ks[2][KS];
+    uint32_t v[8][VW];
+    uint32_t vs[8];
+};
+
+template <int QDT, int PM, int D, int MODE>
+__global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, const Mx4Scales x) {
+    static_assert(PM == PM_TILE || PM == PM_ROW, "page numbers per tile of 16 tokens, or per row");
+    using P2 = Pack2<QDT>;
+    using T = Mx4Tile<D>;
+    constexpr int DV = D;
+    constexpr int DB = D / 16;                 // column blocks of O^T, values of a V row per lane
+    constexpr int KSTEPS = D / 32;             // MFMA steps of a K row
+    constexpr int kTileHeads = 16;
+    constexpr bool kOneSegment = false;        // (fdk_splitkv_mfma_work.h: no single-launch form, units mapped to XCDs)
+    constexpr bool kRowsShareLines = true;
+    constexpr bool kFirstPieceStraight = true;
+    extern __shared__ __attribute__((aligned(16))) char lds[];      // [nw][D * 64] then m[nw][16], l[nw][16], s_next
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int a = lane >> 4;
+    const int c = lane & 15;
+    const int nw = p.wavefronts;
+    const int nh = 1, hl = 0;                  // one kv head per workgroup
+    const int tix = wave;
+    constexpr int kScratch = D * 64;           // a wavefront's 16 output rows in fp32
+    float* sm_m = reinterpret_cast<float*>(lds + nw * kScratch);
+    float* sm_l = sm_m + nw * 16;
+    int* const s_next = reinterpret_cast<int*>(sm_l + nw * 16);
+
+    // out = 0, lse = -inf for the q heads [head0, head0 + heads_here) of an empty sequence; one wavefront
+    auto write_empty_rows = [&](const int b, const int head0, const int heads_here) {
+        for (int idx = lane; idx < heads_here * DV; idx += 64) {
+            const int g = idx / DV, d = idx % DV;
+            const int64_t ob = (int64_t)b * p.out_sb + (int64_t)(head0 + g) * p.out_sh;
+            store_out(p.out, ob + d, 0.f, p.out_dtype);
+            if (d == 0) {
+                if (p.lse) p.lse[(int64_t)b * p.lse_sb + head0 + g] = -INFINITY;
+                if (p.pack_lse) store_out(p.out, ob + DV, -INFINITY, p.out_dtype);
+            }
+        }
+    };
+
+    // One piece: tokens [c_start, min(c_limit, kv_len)) of sequence b for kv head kvh and q-head tile ht; c_start is a
+    // multiple of 16.  Partial results of head g of the tile go to row prow0 + g * prow_step of the workspace.
+    auto run_piece = [&](const int b, const int kvh, const int ht, const int c_start, const int c_limit, const int64_t prow0,
+                         const int prow_step, MergeRows) {
+    const int head0 = kvh * p.group + ht * kTileHeads;
+    const int heads_here = min(kTileHeads, p.group - ht * kTileHeads);
+    // Q^T: lane (h = c, a) holds q[h][(D/4) a + 8 ks .. + 7] (columns past the group repeat its last head, and are not stored)
+    uint4 qb[KSTEPS];
+    {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb +
+                             (int64_t)(head0 + min(c, heads_here - 1)) * p.q_sh + (D / 4) * a;
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) qb[ks] = *reinterpret_cast<const uint4*>(qp + 8 * ks);
+    }
+    const ConstI32 tbl = as_const(p.block_table + (int64_t)b * p.tbl_sb);
+    const int pmask = p.page_size - 1;
+    // Page numbers of a step: one per 16 tokens, wave-uniform; or (any page size) lane l has the one of token l mod 32.
+    struct Pages { int32_t pg[PM == PM_TILE ? 2 : 1]; };
+    auto page_of_token = [&](int n) { return tbl[p.page_shift < 0 ? n / p.page_size : n >> p.page_shift]; };
+    auto fetch_pages = [&](int t, int last, Pages& pi) {     // positions clamped to `last`
+        const int tok0 = c_start + t * kStep;
+        if constexpr (PM == PM_TILE) {
+            pi.pg[0] = tbl[min(tok0, last) >> p.page_shift];
+            pi.pg[1] = tbl[min(tok0 + 16, last) >> p.page_shift];
+        } else {
+            pi.pg[0] = page_of_token(min(tok0 + (lane & 31), last));
+        }
+    };
+    // (ahead of kv_len: clamped to the table, the entries behind the sequence's end are fetched but never used)
+    Pages pa, pb;
+    fetch_pages(tix, p.max_tokens - 1, pa);
+    fetch_pages(tix + nw, p.max_tokens - 1, pb);
+    const int kv_len = min(as_const(p.kv_lens)[b], p.max_tokens);
+    if (c_start >= kv_len) {
+        if (p.direct && tix == 0) write_empty_rows(b, head0, heads_here);
+        return;
+    }
+    const int c_end = min(c_limit, kv_len);
+    const bool softcap = p.soft_cap > 0.f;
+    const float inv_cap = softcap ? 1.0f / p.soft_cap : 0.f;
+
+    const char* kplane = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh;
+    const char* vplane = reinterpret_cast<const char*>(p.v) + (int64_t)kvh * p.v_sh;
+    const char* ksplane = reinterpret_cast<const char*>(x.k) + (int64_t)kvh * x.k_sh;
+    const char* vsplane = reinterpret_cast<const char*>(x.v) + (int64_t)kvh * x.v_sh;
+    const int krow = (c >> 2) + 4 * (c & 3);                  // the token (of 16) that row c of S^T belongs to
+    const uint32_t kbyte = (uint32_t)(a * (D / 8)), vbyte = (uint32_t)(c * (D / 32));
+    const uint32_t ksbyte = (uint32_t)((D / 4) * a / kMxBlock), vsbyte = (uint32_t)(DB * c / kMxBlock);
+
+    auto load_k = [&](const char* at, uint32_t (&dst)[T::KW]) {
+        if constexpr (D == 64) {
+            const uint2 w = *reinterpret_cast<const uint2*>(at);
+            dst[0] = w.x; dst[1] = w.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < T::KW; j += 4) {
+                const uint4 w = *reinterpret_cast<const uint4*>(at + 4 * j);
+                dst[j] = w.x; dst[j + 1] = w.y; dst[j + 2] = w.z; dst[j + 3] = w.w;
+            }
+        }
+    };
+    auto load_v = [&](const char* at, uint32_t (&dst)[T::VW]) {
+        if constexpr (D == 64) {
+            dst[0] = *reinterpret_cast<const uint16_t*>(at);
+        } else if constexpr (D == 128) {
+            dst[0] = *reinterpret_cast<const uint32_t*>(at);
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(at);
+            dst[0] = w.x; dst[1] = w.y;
+        }
+    };
+    // per-lane byte offsets of a tile's rows from its first row (PM_TILE)
+    uint32_t voff[4], vsoff[4];
+    const uint32_t koff = (uint32_t)(krow * p.k_st) + kbyte;
+    const uint32_t ksoff = (uint32_t)(krow * x.k_st) + ksbyte;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        voff[i] = (uint32_t)((a + 4 * i) * p.v_st) + vbyte;
+        vsoff[i] = (uint32_t)((a + 4 * i) * x.v_st) + vsbyte;
+    }
+    // rows of step t; CLAMP: positions past c_end repeat the last token (the partial last step)
+    auto issue = [&](int t, const Pages& pi, T& r, auto clamp_tag) {
+        constexpr bool CLAMP = decltype(clamp_tag)::value;
+        const int tok0 = c_start + t * kStep;
+        if constexpr (PM == PM_TILE && !CLAMP) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int64_t pg = pi.pg[hf];
+                const int64_t slot = (tok0 + 16 * hf) & pmask;
+                const char* kp = kplane + pg * p.k_sp + slot * p.k_st;
+                const char* ksp = ksplane + pg * x.k_sp + slot * x.k_st;
+                load_k(kp + koff, r.k[hf]);
+#pragma unroll
+                for (int g = 0; g < T::KS; ++g) r.ks[hf][g] = *reinterpret_cast<const uint8_t*>(ksp + ksoff + g);
+            }
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int64_t pg = pi.pg[hf];
+                const int64_t slot = (tok0 + 16 * hf) & pmask;
+                const char* vp = vplane + pg * p.v_sp + slot * p.v_st;
+                const char* vsp = vsplane + pg * x.v_sp + slot * x.v_st;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    load_v(vp + voff[i], r.v[4 * hf + i]);
+                    r.vs[4 * hf + i] = *reinterpret_cast<const uint8_t*>(vsp + vsoff[i]);
+                }
+            }
+        } else {
+            // a row's page and slot; row = 0 .. 31 of the step
+            auto place = [&](int row, uint32_t& pg, uint32_t& slot) {
+                int n = tok0 + row;
+                if (CLAMP) n = min(n, c_end - 1);
+                slot = (uint32_t)(p.page_shift < 0 ? n % p.page_size : (n & pmask));
+                if constexpr (PM == PM_TILE) pg = (uint32_t)(row < 16 ? pi.pg[0] : pi.pg[PM == PM_TILE ? 1 : 0]);
+                else pg = (uint32_t)__shfl(pi.pg[0], row, 64);
+            };
+            // (page strides and in-page offsets are below 4 GiB: one 32 x 32 -> 64 bit multiply-add per address)
+            auto at = [&](const char* plane, int64_t sp, int64_t st, uint32_t pg, uint32_t slot) {
+                return plane + ((uint64_t)pg * (uint32_t)sp + (uint64_t)(slot * (uint32_t)st));
+            };
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                uint32_t pg, slot;
+                place(16 * hf + krow, pg, slot);
+                load_k(at(kplane, p.k_sp, p.k_st, pg, slot) + kbyte, r.k[hf]);
+#pragma unroll
+                for (int g = 0; g < T::KS; ++g)
+                    r.ks[hf][g] = *reinterpret_cast<const uint8_t*>(at(ksplane, x.k_sp, x.k_st, pg, slot) + ksbyte + g);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t pg, slot;
+                place(16 * (j >> 2) + a + 4 * (j & 3), pg, slot);
+                load_v(at(vplane, p.v_sp, p.v_st, pg, slot) + vbyte, r.v[j]);
+                r.vs[j] = *reinterpret_cast<const uint8_t*>(at(vsplane, x.v_sp, x.v_st, pg, slot) + vsbyte);
+            }
+        }
+    };
+
+    float m_run = -INFINITY, l_run = 0.f;       // for head c; l_run is this lane group's share of the sum
+    f32x4_t acc[DB];                             // acc[db][i] = O[h = c][DB (4 a + i) + db]
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    auto mma = [&](uint4 av, uint4 bv, f32x4_t cv) { return Mma<QDT>::qk(av, bv, cv); };     // 16 x 16 x 32
+    auto compute = [&](int t, const T& r, auto masked_tag) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
+        // ---- S^T[token][head] = K Q^T, two tiles of 16 tokens ----
+        float sv[8];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks) {
+                const float sc = mx_scale(r.ks[hf][T::KS == 2 ? ks / 4 : 0]);
+                const uint32_t w = r.k[hf][ks];
+                s = mma(make_uint4(mx_unpack2<QDT, 0>(w, sc), mx_unpack2<QDT, 1>(w, sc), mx_unpack2<QDT, 2>(w, sc),
+                                   mx_unpack2<QDT, 3>(w, sc)), qb[ks], s);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sv[4 * hf + i] = s[i];
+        }
+        // ---- online softmax for head c over this lane group's eight tokens ----
+        if (softcap) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sv[i] = soft_cap_fn(sv[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sv[i] *= p.scale_log2;
+        }
+        if (MASKED) {
+            const int tok0 = c_start + t * kStep;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (tok0 + 16 * (i >> 2) + a + 4 * (i & 3) >= c_end) sv[i] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+        mx = max_across_rows(mx);
+        // The running maximum moves only when a step exceeds it by more than 2^8: probabilities of up to 256 are as exact
+        // in 16 bits and in the fp32 sums as those below 1, and the accumulators are rescaled a few times per piece.
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.0f) != 0) {
+            const float m_new = fmaxf(m_run, mx);
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+            m_run = m_new;
+        }
+        float pr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(sv[i] - m_run);
+        l_run += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+        // probabilities rounded to the q dtype, as the 16-bit kernels do; the sum above is of the unrounded ones
+        const uint4 pv = make_uint4(P2::pack(pr[0], pr[1]), P2::pack(pr[2], pr[3]), P2::pack(pr[4], pr[5]), P2::pack(pr[6], pr[7]));
+        // ---- O^T[value][head] += V^T P^T ----
+        float sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = mx_scale(r.vs[j]);
+        auto pair = [&](auto byte_tag, int w, int db) {        // column blocks db, db + 1: byte `byte_tag` of the V words
+            constexpr int BY = decltype(byte_tag)::value;
+            uint32_t u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = mx_unpack2<QDT, BY>(r.v[j][w], sc[j]);
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x05040100u);
+                hi[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
+            }
+            acc[db] = mma(make_uint4(lo[0], lo[1], lo[2], lo[3]), pv, acc[db]);
+            acc[db + 1] = mma(make_uint4(hi[0], hi[1], hi[2], hi[3]), pv, acc[db + 1]);
+        };
+#pragma unroll
+        for (int w = 0; w < T::VW; ++w) {
+            pair(IntTag<0>(), w, 8 * w);
+            pair(IntTag<1>(), w, 8 * w + 2);
+            if constexpr (D >= 128) {
+                pair(IntTag<2>(), w, 8 * w + 4);
+                pair(IntTag<3>(), w, 8 * w + 6);
+            }
+        }
+    };
+
+    // ---- pipeline: two register buffers, the next step's rows are requested before a step is worked on; page numbers run
+    // a step further ahead ----
+    const int n_full = (c_end - c_start) / kStep;
+    {
+        T ra, rb;
+        int t = tix;
+        const int st = nw;
+        if (t < n_full) issue(t, pa, ra, BoolTag<false>());
+        while (t + 2 * st < n_full) {
+            fetch_pages(t + 2 * st, p.max_tokens - 1, pa);
+            issue(t + st, pb, rb, BoolTag<false>());
+            compute(t, ra, BoolTag<false>());
+            fetch_pages(t + 3 * st, p.max_tokens - 1, pb);
+            issue(t + 2 * st, pa, ra, BoolTag<false>());
+            compute(t + st, rb, BoolTag<false>());
+            t += 2 * st;
+        }
+        if (t + st < n_full) {
+            issue(t + st, pb, rb, BoolTag<false>());
+            compute(t, ra, BoolTag<false>());
+            compute(t + st, rb, BoolTag<false>());
+        } else if (t < n_full) {
+            compute(t, ra, BoolTag<false>());
+        }
+        if (n_full * kStep < c_end - c_start && n_full % nw == tix) {
+            fetch_pages(n_full, c_end - 1, pa);
+            issue(n_full, pa, ra, BoolTag<true>());
+            compute(n_full, ra, BoolTag<true>());
+        }
+    }
+
+    // ---- merge: lane groups (sum of l), then the wavefronts through LDS ----
+    // Block e = i (DB / 4) + q of a wavefront's scratch holds, per lane, its values DB (4 a + i) + 4 q .. + 3 of head c: every
+    // LDS instruction touches one contiguous kilobyte, and a merging lane stores four consecutive values.
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    const bool live = c < heads_here;
+    float4* my_o = reinterpret_cast<float4*>(lds + wave * kScratch);
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int q = 0; q < DB / 4; ++q)
+                my_o[(i * (DB / 4) + q) * 64 + lane] = make_float4(acc[4 * q][i], acc[4 * q + 1][i], acc[4 * q + 2][i], acc[4 * q + 3][i]);
+        if (a == 0) {
+            sm_m[wave * 16 + c] = m_run;
+            sm_l[wave * 16 + c] = l_run;
+        }
+    }
+    __syncthreads();
+    if (live) {
+        const int hq = head0 + c;
+        float lse_nat = 0.f;
+        auto merge = [&](auto share_tag) {
+            constexpr int TI = decltype(share_tag)::value;
+            float mw[TI], lw[TI];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < TI; ++t) {
+                mw[t] = sm_m[t * 16 + c];
+                lw[t] = sm_l[t * 16 + c];
+                mx = fmaxf(mx, mw[t]);
+            }
+            float sc[TI], l = 0.f;
+#pragma unroll
+            for (int t = 0; t < TI; ++t) {
+                sc[t] = fast_exp2(mw[t] - mx);               // mx is finite: the piece holds a token
+                l += lw[t] * sc[t];
+            }
+            const float norm = fast_rcp(l);
+            lse_nat = (mx + fast_log2(l)) * kLn2;
+#pragma unroll
+            for (int t = 0; t < TI; ++t) sc[t] *= norm;
+            for (int e = wave; e < DB; e += TI) {
+                float4 xw[TI];
+#pragma unroll
+                for (int t = 0; t < TI; ++t) xw[t] = reinterpret_cast<const float4*>(lds + t * kScratch)[e * 64 + lane];
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int t = 0; t < TI; ++t) {
+                    o.x += xw[t].x * sc[t];
+                    o.y += xw[t].y * sc[t];
+                    o.z += xw[t].z * sc[t];
+                    o.w += xw[t].w * sc[t];
+                }
+                const int d0 = DB * (4 * a + e / (DB / 4)) + 4 * (e % (DB / 4));
+                if (p.direct) store_out4(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + d0, o, p.out_dtype);
+                else *reinterpret_cast<float4*>(p.part_o + (prow0 + (int64_t)c * prow_step) * DV + d0) = o;
+            }
+        };
+        if (nw == 8) merge(IntTag<8>());
+        else merge(IntTag<4>());
+        if (wave == 0 && a == 0) {
+            if (p.direct) {
+                if (p.lse) p.lse[(int64_t)b * p.lse_sb + hq] = lse_nat;
+                if (p.pack_lse) store_out(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + DV, lse_nat, p.out_dtype);
+            } else {
+                p.part_lse[prow0 + (int64_t)c * prow_step] = lse_nat;
+            }
+        }
+    }
+    };   // run_piece
+#include "fdk_splitkv_mfma_work.h"
+}
+
+// (one piece per workgroup or equal shares: a call with counters runs one workgroup per piece, too)
+template <int QDT, int D>
+int launch_mx4(const SplitParams& p_in, const Mx4Scales& x, hipStream_t stream) {
+    SplitParams p = p_in;
+    if (p.fused || p.probe || p.hg_per_wg != 1) return (int)hipErrorInvalidValue;
+    p.head_tiles = (p.group + 15) / 16;
+    p.hg_blocks = p.hkv;
+    p.persistent = 0;
+    const unsigned units = (unsigned)(p.hg_blocks * p.head_tiles);
+    const dim3 grid = p.balanced ? dim3(units, (unsigned)p.workgroups / units) : dim3(units, (unsigned)p.num_splits, (unsigned)p.batch);
+    p.shares = (int32_t)grid.y;
+    p.grid_x = (int32_t)grid.x;
+    const int nw = 8;
+    p.wavefronts = nw;
+    const size_t lds_bytes = (size_t)nw * (D * 64 + 2 * 16 * sizeof(float)) + 16;
+    const int pm = (p.page_shift >= 0 && p.page_size % 16 == 0) ? PM_TILE : PM_ROW;
+#define FDK_MX4_LAUNCH(PMV, MODEV)                                                                                            \
+    do {                                                                                                                      \
+        if (lds_bytes > 64 * 1024) {                                                                                          \
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&splitkv_mx4_kernel<QDT, PMV, D, MODEV>),  \
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes);             \
+            if (e != hipSuccess) return (int)e;                                                                               \
+        }                                                                                                                     \
+        hipLaunchKernelGGL((splitkv_mx4_kernel<QDT, PMV, D, MODEV>), grid, dim3(64 * nw), lds_bytes, stream, p, x);           \
+    } while (0)
+    if (p.balanced) {
+        if (pm == PM_TILE) FDK_MX4_LAUNCH(PM_TILE, WM_SHARES);
+        else FDK_MX4_LAUNCH(PM_ROW, WM_SHARES);
+    } else {
+        if (pm == PM_TILE) FDK_MX4_LAUNCH(PM_TILE, WM_ONE);
+        else FDK_MX4_LAUNCH(PM_ROW, WM_ONE);
+    }
+#undef FDK_MX4_LAUNCH
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+}  // namespace fdk

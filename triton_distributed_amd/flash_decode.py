@@ -40,13 +40,18 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from ._lib import FdkCombineRanksArgs, FdkDecodeArgs, FdkKvAppendArgs, FdkMeasureArgs, FdkPlan
+from ._lib import FdkCombineRanksArgs, FdkDecodeArgs, FdkKvAppendArgs, FdkMeasureArgs, FdkMxfp4Args, FdkPlan
 
 _LIB = _lib.load()          # raises ImportError when libfdk.so is not built - by design
 
 _TORCH_TO_FDK = {torch.bfloat16: _lib.FDK_BF16, torch.float16: _lib.FDK_FP16, torch.float32: _lib.FDK_FP32}
 if hasattr(torch, "float8_e4m3fn"):
     _TORCH_TO_FDK[torch.float8_e4m3fn] = _lib.FDK_FP8_E4M3
+# MXFP4 rows: packed e2m1 codes, two values an element (either spelling of the type), scales as bytes or as e8m0
+_MXFP4_CODES = {torch.uint8} | ({torch.float4_e2m1fn_x2} if hasattr(torch, "float4_e2m1fn_x2") else set())
+_MXFP4_SCALES = {torch.uint8} | ({torch.float8_e8m0fnu} if hasattr(torch, "float8_e8m0fnu") else set())
+MXFP4_BLOCK = 32
+_TORCH_TO_FDK.update({t: _lib.FDK_MXFP4 for t in _MXFP4_CODES})
 _ALGOS = {"auto": _lib.FDK_ALGO_AUTO, "valu": _lib.FDK_ALGO_VALU, "mfma": _lib.FDK_ALGO_MFMA}
 _ALGO_NAMES = {v: k for k, v in _ALGOS.items()}
 
@@ -56,6 +61,23 @@ def _fdk_dtype(t: torch.dtype, what: str) -> int:
         return _TORCH_TO_FDK[t]
     except KeyError:
         raise ValueError(f"{what}: unsupported dtype {t}") from None
+
+
+def _row_values(cache: torch.Tensor) -> int:
+    """Values of a cache row: the last axis, twice that of packed 4-bit codes."""
+    return cache.shape[-1] * (2 if cache.dtype in _MXFP4_CODES else 1)
+
+
+def _check_block_scales(name: str, scale: Optional[torch.Tensor], cache: torch.Tensor) -> None:
+    """The scale bytes of an MXFP4 cache: the cache's shape with one byte per block of 32 values in the last axis."""
+    want = tuple(cache.shape[:-1]) + (_row_values(cache) // MXFP4_BLOCK,)
+    if scale is None:
+        raise ValueError(f"{name} is required for an MXFP4 cache: the block scales, uint8 {list(want)}")
+    if scale.dtype not in _MXFP4_SCALES or tuple(scale.shape) != want or scale.stride(-1) != 1:
+        raise ValueError(f"{name} must hold the block scales of an MXFP4 cache, uint8 (or e8m0) {list(want)} with a contiguous "
+                         f"last axis; got {scale.dtype} {list(scale.shape)}")
+    if scale.device != cache.device:
+        raise ValueError(f"{name} is on {scale.device}, its cache on {cache.device}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -134,11 +156,12 @@ def _fill_args(q, k_cache, v_cache, block_table, kv_lens, sm_scale, soft_cap, kv
     if k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("k_cache / v_cache must be [num_pages, page_size, kv_heads, head_dim]")
     batch, q_heads, q_head_dim = q.shape
-    _, page_size, kv_heads, k_head_dim = k_cache.shape
+    _, page_size, kv_heads, _ = k_cache.shape
+    k_head_dim = _row_values(k_cache)
     # the reference's shape asserts, flash_decode.py:851,860
     assert page_size == v_cache.shape[1] and kv_heads == v_cache.shape[2] and k_head_dim == q_head_dim
     assert q_heads % kv_heads == 0
-    v_head_dim = v_cache.shape[-1]       # (the reference: V_DIM next to K_DIM, flash_decode.py:103-109; the library says what is built)
+    v_head_dim = _row_values(v_cache)    # (the reference: V_DIM next to K_DIM, flash_decode.py:103-109; the library says what is built)
     if k_cache.dtype != v_cache.dtype:
         raise ValueError("k_cache and v_cache must share a dtype")
     if q.stride(-1) != 1 or k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
@@ -172,8 +195,15 @@ def _fill_args(q, k_cache, v_cache, block_table, kv_lens, sm_scale, soft_cap, kv
             if s is not None and (s.dtype != torch.float32 or s.numel() != kv_heads or not s.is_contiguous()):
                 raise ValueError(f"{name} must be a contiguous fp32 tensor of {kv_heads} per-kv-head scales")
         a.k_scale, a.v_scale = _ptr(k_scale), _ptr(v_scale)
+    elif a.kv_dtype == _lib.FDK_MXFP4:
+        if k_scale is not None or v_scale is not None or check_device:     # (a plan alone needs none)
+            _check_block_scales("k_scale", k_scale, k_cache)
+            _check_block_scales("v_scale", v_scale, v_cache)
+            a.kbs_stride_page, a.kbs_stride_tok, a.kbs_stride_head = k_scale.stride()[:3]
+            a.vbs_stride_page, a.vbs_stride_tok, a.vbs_stride_head = v_scale.stride()[:3]
+            a.k_block_scale, a.v_block_scale = k_scale.data_ptr(), v_scale.data_ptr()
     elif k_scale is not None or v_scale is not None:
-        raise ValueError("k_scale / v_scale are only meaningful for an fp8 KV cache")
+        raise ValueError("k_scale / v_scale are only meaningful for an fp8 or MXFP4 KV cache")
     a.block_table = block_table.data_ptr()
     a.table_stride_b = block_table.stride(0) if batch > 1 else max(block_table.stride(0), block_table.shape[1])
     a.kv_lens = kv_lens.data_ptr()
@@ -218,10 +248,13 @@ def _args_and_plan(q, k_cache, v_cache, block_table, kv_lens, sm_scale, soft_cap
     a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     a.block_table, a.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
     a.max_kv_len, a.min_kv_len = bounds
-    if k_scale is not None:
-        a.k_scale = k_scale.data_ptr()
-    if v_scale is not None:
-        a.v_scale = v_scale.data_ptr()
+    if a.kv_dtype == _lib.FDK_MXFP4:
+        a.k_block_scale, a.v_block_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    else:
+        if k_scale is not None:
+            a.k_scale = k_scale.data_ptr()
+        if v_scale is not None:
+            a.v_scale = v_scale.data_ptr()
     plan = hit[1].get(bounds)
     if plan is None:
         plan = _plan_of(a)                      # (also where the library refuses the bounds)
@@ -409,7 +442,7 @@ def prepare_decode(q, k_cache, v_cache, block_table, kv_lens, sm_scale, *, soft_
         q, k_cache, v_cache, block_table, kv_lens, sm_scale, soft_cap, kv_split, max_kv_len, k_scale, v_scale, algo,
         min_kv_len)
     batch, q_heads = q.shape[:2]
-    d = v_cache.shape[-1]                     # values of an output row: V's head dim (the reference's V_DIM)
+    d = _row_values(v_cache)                  # values of an output row: V's head dim (the reference's V_DIM)
     measure = None
     if wavefronts or buffers or shares_per_cu or probe_loads or rotate_heads or force_balanced or timeline is not None:
         measure = FdkMeasureArgs()
@@ -496,7 +529,8 @@ def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     """Local (one GPU's share) split-KV GQA decode attention over a paged KV cache.
 
     q            [B, Hq, D] bf16/fp16, one query token per sequence
-    k_cache      [num_pages, P, Hkv, D] in q's dtype or float8_e4m3fn
+    k_cache      [num_pages, P, Hkv, D] in q's dtype or float8_e4m3fn; or MXFP4 codes [num_pages, P, Hkv, D/2]
+                 (float4_e2m1fn_x2 or uint8: value 2i in the low four bits of byte i)
     v_cache      same shape and dtype as k_cache
     block_table  [B, max_pages] int32: page of token n is ``block_table[b, n // P]``, slot ``n % P``
     kv_lens      [B] int32 (device tensor; never read on the host)
@@ -510,7 +544,8 @@ def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
                  per-sequence chunks of one size); otherwise long contexts of two or more sequences are cut into
                  equal shares of the tokens on the device (a single pass is as slow as its longest sequence) and
                  per-sequence chunks follow each sequence's own length; results never depend on it
-    k_scale/v_scale  [Hkv] fp32 dequantisation scales of an fp8 cache
+    k_scale/v_scale  [Hkv] fp32 dequantisation scales of an fp8 cache; of an MXFP4 cache its e8m0 block scales
+                     [num_pages, P, Hkv, D/32] (uint8 or float8_e8m0fnu, value = code * 2^(byte - 127))
     fp8_fold_k_scale fp8 cache: apply k_scale to the logits instead of to every K value (see ``prepare_decode``)
     force_balanced   measurement / test aid: equal shares of the whole batch whatever the planner would choose
 
@@ -866,3 +901,75 @@ def probe_linear_read(buf: torch.Tensor, nontemporal: bool = True, workgroups: i
         raise ValueError("buf must be a contiguous GPU tensor")
     _lib.check(_LIB.fdk_probe_linear_read(buf.data_ptr(), buf.numel() * buf.element_size(), int(bool(nontemporal)),
                                           int(workgroups), _stream_handle(stream)))
+
+
+def _row_axes(*tensors: torch.Tensor):
+    """Sizes and strides of the three row axes of tensors [..., last] that share their leading shape: axes that lie
+    contiguously in every tensor are merged."""
+    lead = list(zip(tensors[0].shape[:-1], *(t.stride()[:-1] for t in tensors)))
+    merged = []
+    for n, *st in lead:
+        if n == 1:
+            continue
+        if merged and all(ps == n * s for ps, s in zip(merged[-1][1:], st)):
+            merged[-1] = [merged[-1][0] * n] + st
+        else:
+            merged.append([n] + st)
+    if len(merged) > 3:
+        raise ValueError("at most three row axes that do not merge")
+    merged = [[1] + [0] * len(tensors)] * (3 - len(merged)) + merged
+    return [m[0] for m in merged], [[m[1 + i] for m in merged] for i in range(len(tensors))]
+
+
+def _mxfp4_convert(fn, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, stream) -> None:
+    d = x.shape[-1]
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"MXFP4 rows are converted from and to bf16 / fp16, not {x.dtype}")
+    if d == 0 or d % MXFP4_BLOCK:
+        raise ValueError(f"rows must hold a multiple of {MXFP4_BLOCK} values, got {d}")
+    if codes.dtype not in _MXFP4_CODES or tuple(codes.shape) != tuple(x.shape[:-1]) + (d // 2,):
+        raise ValueError(f"codes must be uint8 (or float4_e2m1fn_x2) {list(x.shape[:-1]) + [d // 2]}, got {codes.dtype} {list(codes.shape)}")
+    _check_block_scales("scales", scales, codes)
+    for name, t in (("x", x), ("codes", codes)):
+        if not t.is_cuda:
+            raise ValueError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
+        if t.stride(-1) != 1:
+            raise ValueError(f"the last axis of {name} must be contiguous")
+    if x.device != codes.device:
+        raise ValueError(f"codes is on {codes.device}, x on {x.device}")
+    if x.numel() == 0:
+        return
+    n, (xs, cs, ss) = _row_axes(x, codes, scales)
+    a = FdkMxfp4Args()
+    a.struct_size = C.sizeof(FdkMxfp4Args)
+    a.x, a.codes, a.scales = x.data_ptr(), codes.data_ptr(), scales.data_ptr()
+    if max(n) > 2 ** 31 - 1:
+        raise ValueError("too many rows")
+    a.n, a.x_stride, a.codes_stride, a.scales_stride = (C.c_int32 * 3)(*n), (C.c_int64 * 3)(*xs), (C.c_int64 * 3)(*cs), (C.c_int64 * 3)(*ss)
+    a.num_values, a.x_dtype = d, _fdk_dtype(x.dtype, "x")
+    _lib.check(fn(C.byref(a), _stream_handle(stream)))
+
+
+def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,
+                   stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 / fp16 rows ``[..., D]`` as MXFP4: ``(codes [..., D/2] uint8, scales [..., D/32] uint8)`` - what the append
+    writes into an MXFP4 cache, e.g. to convert a cache that exists in 16 bits.
+
+    The scale of a block of 32 values is the smallest power of two with amax <= 7 scales, within [2^-126, 2^125] for bf16
+    and [2^-126, 2^13] for fp16; codes are rounded to nearest, ties to even, and saturate at 6 scales.  A block with an
+    infinity or a NaN in it reads as NaN (scale byte 255)."""
+    if codes is None:
+        codes = torch.empty(x.shape[:-1] + (x.shape[-1] // 2,), dtype=torch.uint8, device=x.device)
+    if scales is None:
+        scales = torch.empty(x.shape[:-1] + (x.shape[-1] // MXFP4_BLOCK,), dtype=torch.uint8, device=x.device)
+    _mxfp4_convert(_LIB.fdk_mx_quantize, x, codes, scales, stream)
+    return codes, scales
+
+
+def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16, *,
+                     out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """The values MXFP4 rows stand for, ``code * 2^(scale byte - 127)``, as bf16 / fp16 ``[..., D]``."""
+    if out is None:
+        out = torch.empty(codes.shape[:-1] + (codes.shape[-1] * 2,), dtype=dtype, device=codes.device)
+    _mxfp4_convert(_LIB.fdk_mx_dequantize, out, codes, scales, stream)
+    return out
