@@ -277,7 +277,7 @@ typedef struct fdk_kv_append_args {
     const void* qkv;      /* [B, T, Hq + 2 Hkv, D]: q heads, then k heads, then v heads */
     int64_t qkv_stride_b, qkv_stride_t, qkv_stride_h;
     int32_t qkv_dtype;    /* FDK_BF16 | FDK_FP16 (also of the weights and of q_out) */
-    int32_t kv_dtype;     /* = qkv_dtype, or FDK_FP8_E4M3 */
+    int32_t kv_dtype;     /* = qkv_dtype, or FDK_FP8_E4M3 (fdk_kv_append_axes: also FDK_MXFP4) */
     const void* q_weight; /* [D] RMSNorm weight of the q heads */
     const void* k_weight; /* [D] RMSNorm weight of the k heads */
     float q_eps, k_eps;
@@ -300,6 +300,29 @@ typedef struct fdk_kv_append_args {
     void* q_out;          /* [B, T, Hq, D] */
     int64_t q_out_stride_b, q_out_stride_t, q_out_stride_h;
 } fdk_kv_append_args;
+
+/* (revision 3) The append with explicit positions, and into an MXFP4 cache: the block of fdk_kv_append and what it lacks.
+ *   Positions: pair i of a row (y[i], y[i + D/2]) turns by row positions[axis(i), b, t] of the cos / sin tables instead of row
+ * pos - a cache from which tokens were evicted, where a token's place is not its position, or positions of several axes
+ * (time, height, width).  rope_sections[x] pairs belong to axis x and add up to D/2: one section after the other, or, with
+ * rope_interleaved, pair i to axis i mod num_axes while i / num_axes < rope_sections[that axis] and to axis 0 otherwise.
+ * Where K / V rows go is still decided by kv_lens.
+ *   MXFP4 (append->kv_dtype = FDK_MXFP4): the caches' rows are D/2 bytes with strides in bytes, 2-byte aligned; they receive
+ * the codes and scales that fdk_mx_quantize gives for the 16-bit values a 16-bit cache would have received. */
+typedef struct fdk_kv_append_axes_args {
+    uint32_t struct_size;     /* = sizeof(fdk_kv_append_axes_args) */
+    uint32_t flags;           /* FDK_FLAG_DRY_RUN (here or in *append) */
+    const fdk_kv_append_args* append;
+    const int32_t* positions; /* [num_axes, B, T], strides in elements; null: the tokens' places in the cache */
+    int64_t pos_stride_axis, pos_stride_b, pos_stride_t;
+    int32_t num_axes;         /* 1 .. 4 (0 without positions) */
+    int32_t rope_interleaved;
+    int32_t rope_sections[4];
+    uint8_t* k_block_scale;   /* FDK_MXFP4: [num_pages, P, Hkv, D/32], byte strides of the page, token and head axes */
+    uint8_t* v_block_scale;
+    int64_t kbs_stride_page, kbs_stride_tok, kbs_stride_head;
+    int64_t vbs_stride_page, vbs_stride_tok, vbs_stride_head;
+} fdk_kv_append_axes_args;
 
 /* (revision 3) Conversion between 16-bit rows and MXFP4 rows (see FDK_MXFP4): n0 x n1 x n2 rows of num_values values, each
  * tensor with strides of its three row axes (elements; bytes for codes and scales), values contiguous.
@@ -386,6 +409,9 @@ int fdk_mx_dequantize(const fdk_mxfp4_args* args, void* hip_stream);
 
 /* Normalise, rotate and append the new tokens (see fdk_kv_append_args). */
 int fdk_kv_append(const fdk_kv_append_args* args, void* hip_stream);
+
+/* ... with explicit positions, or into an MXFP4 cache (see fdk_kv_append_axes_args). */
+int fdk_kv_append_axes(const fdk_kv_append_axes_args* args, void* hip_stream);
 
 #ifdef __cplusplus
 }

@@ -6,7 +6,7 @@ import torch
 
 from oracle import mxfp4
 from triton_distributed_amd import _lib
-from triton_distributed_amd._lib import FdkDecodeArgs, FdkMxfp4Args, FdkPlan
+from triton_distributed_amd._lib import FdkDecodeArgs, FdkKvAppendArgs, FdkKvAppendAxesArgs, FdkMxfp4Args, FdkPlan
 import triton_distributed_amd as tda
 
 
@@ -154,3 +154,72 @@ def test_oracle_by_hand():
     assert mxfp4.quantize(x)[1].tolist() == [[255, 128]]
     assert mxfp4.quantize(torch.full((1, 32), 65504.0, dtype=torch.float16))[1].tolist() == [[127 + 13]]
     assert mxfp4.quantize(torch.zeros(1, 32, dtype=torch.float16))[1].tolist() == [[1]]
+
+
+def _append_args(kw):
+    """A valid dry-run fdk_kv_append block on fake pointers: B32, 1 new token, 32q/8kv, D128, P16, 4-bit cache, three axes."""
+    a = FdkKvAppendArgs()
+    a.struct_size = C.sizeof(FdkKvAppendArgs)
+    a.flags = _lib.FDK_FLAG_DRY_RUN
+    a.qkv, a.q_weight, a.k_weight, a.cos, a.sin = 0x10000, 0x20000, 0x30000, 0x40000, 0x50000
+    a.qkv_stride_b, a.qkv_stride_t, a.qkv_stride_h = 48 * 128, 48 * 128, 128
+    a.qkv_dtype, a.kv_dtype = _lib.FDK_BF16, _lib.FDK_MXFP4
+    a.q_eps = a.k_eps = 1e-6
+    a.cs_stride_b, a.cs_stride_pos, a.max_positions = 0, 128, 8192
+    a.batch, a.new_tokens, a.num_q_heads, a.num_kv_heads, a.head_dim = 32, 1, 32, 8, 128
+    a.block_table, a.table_stride_b, a.kv_lens = 0x60000, 256, 0x70000
+    a.page_size, a.max_pages, a.num_pages = 16, 256, 9000
+    a.k_cache, a.v_cache = 0x80000, 0x90000
+    a.k_stride_page = a.v_stride_page = 16 * 8 * 64
+    a.k_stride_tok = a.v_stride_tok = 8 * 64
+    a.k_stride_head = a.v_stride_head = 64
+    a.q_out, a.q_out_stride_b, a.q_out_stride_t, a.q_out_stride_h = 0xA0000, 32 * 128, 32 * 128, 128
+    x = FdkKvAppendAxesArgs()
+    x.struct_size = C.sizeof(FdkKvAppendAxesArgs)
+    x.append = C.addressof(a)
+    x.k_block_scale, x.v_block_scale = 0xB0001, 0xC0001
+    x.kbs_stride_page, x.kbs_stride_tok, x.kbs_stride_head = 16 * 8 * 4, 8 * 4, 4
+    x.vbs_stride_page, x.vbs_stride_tok, x.vbs_stride_head = 16 * 8 * 4, 8 * 4, 4
+    x.positions, x.pos_stride_axis, x.pos_stride_b, x.pos_stride_t = 0xD0000, 32, 1, 1
+    x.num_axes, x.rope_sections = 3, (C.c_int32 * 4)(24, 20, 20, 0)
+    for k, v in kw.items():
+        setattr(x if hasattr(x, k) and k not in ("struct_size", "flags") else a, k, v)
+    return a, x
+
+
+def _append_rc(**kw):
+    a, x = _append_args(kw)
+    return _lib.load().fdk_kv_append_axes(C.byref(x), None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({}, 0), (dict(num_axes=0), _lib.FDK_ESHAPE), (dict(num_axes=5), _lib.FDK_ESHAPE), (dict(num_axes=2), _lib.FDK_ESHAPE),
+    (dict(rope_sections=(C.c_int32 * 4)(64, 20, -20, 0)), _lib.FDK_ESHAPE), (dict(positions=0xD0002), _lib.FDK_EALIGN),
+    (dict(positions=None), _lib.FDK_ENULL), (dict(positions=None, num_axes=0), 0),
+    (dict(positions=None, num_axes=0, rope_interleaved=1), _lib.FDK_ENULL),
+    (dict(k_block_scale=None), _lib.FDK_ENULL), (dict(kbs_stride_head=3), _lib.FDK_ESHAPE), (dict(v_stride_head=63), _lib.FDK_ESHAPE),
+    (dict(k_cache=0x80001), _lib.FDK_EALIGN), (dict(v_stride_tok=8 * 64 + 1), _lib.FDK_EALIGN),
+    (dict(kv_dtype=_lib.FDK_BF16, k_stride_head=128, v_stride_head=128), 0),
+    (dict(kv_dtype=_lib.FDK_FP16), _lib.FDK_EUNSUPPORTED),
+])
+def test_append_refusals(kw, code):
+    assert _append_rc(**kw) == code
+
+
+def test_append_blocks():
+    """The block of fdk_kv_append alone knows no 4-bit rows; the block around it is checked like the others."""
+    lib = _lib.load()
+    a, x = _append_args({})
+    assert lib.fdk_kv_append(C.byref(a), None) == _lib.FDK_EUNSUPPORTED
+    assert lib.fdk_kv_append_axes(None, None) == _lib.FDK_ENULL
+    x.struct_size -= 8
+    assert lib.fdk_kv_append_axes(C.byref(x), None) == _lib.FDK_EABI
+    x.struct_size += 8
+    a.struct_size -= 8
+    assert lib.fdk_kv_append_axes(C.byref(x), None) == _lib.FDK_EABI
+    x.append = None
+    assert lib.fdk_kv_append_axes(C.byref(x), None) == _lib.FDK_ENULL
+    # neither positions nor 4-bit rows: the plain append
+    a, x = _append_args(dict(positions=None, num_axes=0, kv_dtype=_lib.FDK_BF16, k_stride_head=128, v_stride_head=128,
+                             k_block_scale=None))
+    assert lib.fdk_kv_append_axes(C.byref(x), None) == 0

@@ -29,6 +29,7 @@ EXPORTS = (
     "fdk_abi_version", "fdk_abi_revision", "fdk_last_error", "fdk_device_cus", "fdk_plan", "fdk_workspace_bytes",
     "fdk_decode", "fdk_decode_splitkv", "fdk_combine", "fdk_combine_ranks", "fdk_counters_len", "fdk_kv_append",
     "fdk_decode_static", "fdk_length_feedback_alloc", "fdk_length_feedback_free", "fdk_mx_quantize", "fdk_mx_dequantize",
+    "fdk_kv_append_axes",
 )
 # declared in include/fdk_measure.h
 MEASURE_EXPORTS = ("fdk_probe_linear_read",)
@@ -113,6 +114,17 @@ class FdkKvAppendArgs(C.Structure):
     ]
 
 
+class FdkKvAppendAxesArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("flags", C.c_uint32), ("append", C.c_void_p),      # FdkKvAppendArgs*
+        ("positions", C.c_void_p), ("pos_stride_axis", C.c_int64), ("pos_stride_b", C.c_int64), ("pos_stride_t", C.c_int64),
+        ("num_axes", C.c_int32), ("rope_interleaved", C.c_int32), ("rope_sections", C.c_int32 * 4),
+        ("k_block_scale", C.c_void_p), ("v_block_scale", C.c_void_p),
+        ("kbs_stride_page", C.c_int64), ("kbs_stride_tok", C.c_int64), ("kbs_stride_head", C.c_int64),
+        ("vbs_stride_page", C.c_int64), ("vbs_stride_tok", C.c_int64), ("vbs_stride_head", C.c_int64),
+    ]
+
+
 class FdkMxfp4Args(C.Structure):
     _fields_ = [
         ("struct_size", C.c_uint32), ("flags", C.c_uint32),
@@ -174,6 +186,8 @@ def load() -> C.CDLL:
     lib.fdk_length_feedback_free.argtypes = [C.c_void_p]
     lib.fdk_kv_append.restype = C.c_int
     lib.fdk_kv_append.argtypes = [C.POINTER(FdkKvAppendArgs), C.c_void_p]
+    lib.fdk_kv_append_axes.restype = C.c_int
+    lib.fdk_kv_append_axes.argtypes = [C.POINTER(FdkKvAppendAxesArgs), C.c_void_p]
     for name in ("fdk_mx_quantize", "fdk_mx_dequantize"):
         fn = getattr(lib, name)
         fn.restype = C.c_int

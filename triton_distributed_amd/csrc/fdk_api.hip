@@ -862,8 +862,8 @@ int fdk_mx_quantize(const fdk_mxfp4_args* args, void* hip_stream) { return mxfp4
 
 int fdk_mx_dequantize(const fdk_mxfp4_args* args, void* hip_stream) { return mxfp4_convert(args, false, hip_stream); }
 
-int fdk_kv_append(const fdk_kv_append_args* caller_args, void* hip_stream) {
-    g_err[0] = 0;
+// (x: what fdk_kv_append_axes adds, or null)
+static int kv_append(const fdk_kv_append_args* caller_args, const fdk_kv_append_axes_args* x, void* hip_stream) {
     if (!caller_args) return fail(FDK_ENULL, "args is null");
     fdk_kv_append_args local;
     if (int rc = adopt(caller_args, caller_args->struct_size, sizeof(fdk_kv_append_args), "fdk_kv_append_args", &local))
@@ -876,8 +876,9 @@ int fdk_kv_append(const fdk_kv_append_args* caller_args, void* hip_stream) {
         return fail(FDK_EUNSUPPORTED, "head_dim %d not built (64, 128 or 256)", a->head_dim);
     if (a->qkv_dtype != FDK_BF16 && a->qkv_dtype != FDK_FP16)
         return fail(FDK_EUNSUPPORTED, "qkv_dtype %d (bf16 or fp16 only)", a->qkv_dtype);
-    if (a->kv_dtype != a->qkv_dtype && a->kv_dtype != FDK_FP8_E4M3)
-        return fail(FDK_EUNSUPPORTED, "kv_dtype %d must equal qkv_dtype or be fp8_e4m3", a->kv_dtype);
+    const bool mx = x && a->kv_dtype == FDK_MXFP4;
+    if (a->kv_dtype != a->qkv_dtype && a->kv_dtype != FDK_FP8_E4M3 && !mx)
+        return fail(FDK_EUNSUPPORTED, "kv_dtype %d must equal qkv_dtype or be fp8_e4m3 (fdk_kv_append_axes: or mxfp4)", a->kv_dtype);
     if (a->page_size <= 0 || a->max_pages <= 0 || a->num_pages <= 0)
         return fail(FDK_ESHAPE, "page_size %d, max_pages %d, num_pages %d must be positive", a->page_size, a->max_pages,
                     a->num_pages);
@@ -885,6 +886,20 @@ int fdk_kv_append(const fdk_kv_append_args* caller_args, void* hip_stream) {
     if (a->max_positions <= 0) return fail(FDK_ESHAPE, "max_positions %d <= 0", a->max_positions);
     if (!(a->q_eps == a->q_eps) || !(a->k_eps == a->k_eps) || a->q_eps < 0.f || a->k_eps < 0.f)
         return fail(FDK_ESHAPE, "eps must be non-negative numbers");
+    const bool explicit_positions = x && x->positions;
+    if (explicit_positions) {
+        if (x->num_axes < 1 || x->num_axes > 4) return fail(FDK_ESHAPE, "num_axes %d outside [1, 4]", x->num_axes);
+        int64_t pairs = 0;
+        for (int ax = 0; ax < x->num_axes; ++ax) {
+            if (x->rope_sections[ax] < 0) return fail(FDK_ESHAPE, "rope_sections[%d] = %d < 0", ax, x->rope_sections[ax]);
+            pairs += x->rope_sections[ax];
+        }
+        if (pairs != a->head_dim / 2)
+            return fail(FDK_ESHAPE, "rope_sections add up to %lld pairs, a row has %d", (long long)pairs, a->head_dim / 2);
+        if (reinterpret_cast<uintptr_t>(x->positions) & 3u) return fail(FDK_EALIGN, "positions not 4-byte aligned");
+    } else if (x && (x->num_axes || x->rope_interleaved)) {
+        return fail(FDK_ENULL, "num_axes / rope_interleaved without positions");
+    }
     if (a->batch == 0 || a->new_tokens == 0) return FDK_OK;
     const int64_t head_rows = (int64_t)a->num_q_heads + 2 * (int64_t)a->num_kv_heads;
     if ((int64_t)a->batch * a->new_tokens > (int64_t)INT32_MAX * 4 / head_rows)       // one wavefront per head row
@@ -904,9 +919,21 @@ int fdk_kv_append(const fdk_kv_append_args* caller_args, void* hip_stream) {
                            a->v_stride_page, a->v_stride_tok, a->v_stride_head};
     for (int i = 0; i < 6; ++i)
         if (st[i] < 0) return fail(FDK_ESHAPE, "negative cache stride");
-    if (a->num_kv_heads > 1 && (a->k_stride_head < a->head_dim || a->v_stride_head < a->head_dim))
+    const int row_elems = mx ? a->head_dim / 2 : a->head_dim;
+    if (a->num_kv_heads > 1 && (a->k_stride_head < row_elems || a->v_stride_head < row_elems))
         return fail(FDK_ESHAPE, "cache head stride < head_dim");
-    if (a->flags & FDK_FLAG_DRY_RUN) return FDK_OK;
+    if (mx) {
+        if (!x->k_block_scale || !x->v_block_scale)
+            return fail(FDK_ENULL, "k_block_scale / v_block_scale are required for an mxfp4 cache");
+        int rc = check_scale_strides(x->kbs_stride_page, x->kbs_stride_tok, x->kbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
+        if (!rc) rc = check_scale_strides(x->vbs_stride_page, x->vbs_stride_tok, x->vbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
+        if (rc) return rc;
+        int64_t odd = 0;
+        for (int i = 0; i < 6; ++i) odd |= st[i];
+        if (((odd | (int64_t)reinterpret_cast<uintptr_t>(a->k_cache) | (int64_t)reinterpret_cast<uintptr_t>(a->v_cache)) & 1) != 0)
+            return fail(FDK_EALIGN, "rows of an mxfp4 cache must be 2-byte aligned");
+    }
+    if ((a->flags | (x ? x->flags : 0)) & FDK_FLAG_DRY_RUN) return FDK_OK;
     fdk::KvAppendParams p;
     memset(&p, 0, sizeof(p));
     p.qkv = a->qkv; p.q_weight = a->q_weight; p.k_weight = a->k_weight; p.cos = a->cos; p.sin = a->sin;
@@ -920,9 +947,49 @@ int fdk_kv_append(const fdk_kv_append_args* caller_args, void* hip_stream) {
     p.batch = a->batch; p.new_tokens = a->new_tokens; p.hq = a->num_q_heads; p.hkv = a->num_kv_heads;
     p.head_dim = a->head_dim; p.page_size = a->page_size; p.max_pages = a->max_pages; p.num_pages = a->num_pages;
     p.max_positions = a->max_positions; p.q_eps = a->q_eps; p.k_eps = a->k_eps;
-    int rc = fdk::launch_kv_append(p, a->qkv_dtype, a->kv_dtype, reinterpret_cast<hipStream_t>(hip_stream));
+    int rc;
+    if (mx || explicit_positions) {
+        fdk::KvAppendAxes m;
+        memset(&m, 0, sizeof(m));
+        m.positions = x->positions;
+        m.pos_sa = x->pos_stride_axis; m.pos_sb = x->pos_stride_b; m.pos_st = x->pos_stride_t;
+        m.num_axes = explicit_positions ? x->num_axes : 1;
+        m.interleaved = x->rope_interleaved ? 1 : 0;
+        for (int ax = 0, end = 0; ax < 4; ++ax) {
+            if (ax < m.num_axes) end += explicit_positions ? x->rope_sections[ax] : a->head_dim / 2;
+            m.section_end[ax] = ax < m.num_axes ? end : INT32_MAX;
+        }
+        // four values at a time: 8 bytes of the 16-bit tensors, 4 bytes of an fp8 row
+        const int cb = elem_size(a->kv_dtype) * 4;
+        uintptr_t odd = 0;
+        odd |= (reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->q_out)) & 7u;
+        odd |= (uintptr_t)(a->qkv_stride_b | a->qkv_stride_t | a->qkv_stride_h | a->q_out_stride_b | a->q_out_stride_t | a->q_out_stride_h) & 3u;
+        if (!mx) {
+            odd |= (reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & (uintptr_t)(cb - 1);
+            odd |= (uintptr_t)(st[0] | st[1] | st[2] | st[3] | st[4] | st[5]) & 3u;
+        }
+        m.aligned = odd == 0 ? 1 : 0;
+        m.scales = fdk::Mx4Scales{x->k_block_scale,   x->v_block_scale,   x->kbs_stride_page, x->kbs_stride_tok,
+                                  x->kbs_stride_head, x->vbs_stride_page, x->vbs_stride_tok,  x->vbs_stride_head};
+        rc = fdk::launch_kv_append_axes(p, m, a->qkv_dtype, a->kv_dtype, reinterpret_cast<hipStream_t>(hip_stream));
+    } else {
+        rc = fdk::launch_kv_append(p, a->qkv_dtype, a->kv_dtype, reinterpret_cast<hipStream_t>(hip_stream));
+    }
     if (rc) return fail(rc, "kv append launch failed: %s", hipGetErrorString((hipError_t)rc));
     return FDK_OK;
+}
+
+int fdk_kv_append(const fdk_kv_append_args* args, void* hip_stream) {
+    g_err[0] = 0;
+    return kv_append(args, nullptr, hip_stream);
+}
+
+int fdk_kv_append_axes(const fdk_kv_append_axes_args* args, void* hip_stream) {
+    g_err[0] = 0;
+    if (!args) return fail(FDK_ENULL, "args is null");
+    fdk_kv_append_axes_args local;
+    if (int rc = adopt(args, args->struct_size, sizeof(fdk_kv_append_axes_args), "fdk_kv_append_axes_args", &local)) return rc;
+    return kv_append(local.append, &local, hip_stream);
 }
 
 }  // extern "C"

@@ -22,7 +22,19 @@ struct Mx4Scales {
     int64_t v_sp, v_st, v_sh;
 };
 
+// Explicit positions of an append (several axes: each turns its own section of the rotary pairs) and the scales of an MXFP4
+// cache, beside KvAppendParams.
+struct KvAppendAxes {
+    const int32_t* positions;                // [axes, B, T]; null: every pair turns by the token's place in the cache
+    int64_t pos_sa, pos_sb, pos_st;
+    int32_t num_axes, interleaved;
+    int32_t section_end[4];                  // pairs of axes 0 .. x together (INT32_MAX from the last axis on)
+    int32_t aligned;                         // rows may be read and written four values at a time
+    Mx4Scales scales;
+};
+
 // Launchers; return hipError_t as int.
+int launch_kv_append_axes(const KvAppendParams& p, const KvAppendAxes& m, int qkv_dtype, int kv_dtype, hipStream_t stream);
 int launch_splitkv_mx4(const SplitParams& p, const Mx4Scales& x, int q_dtype, hipStream_t stream);
 int launch_mxfp4(const fdk_mxfp4_args& a, bool quantize, hipStream_t stream);
 

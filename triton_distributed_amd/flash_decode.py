@@ -40,7 +40,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from ._lib import FdkCombineRanksArgs, FdkDecodeArgs, FdkKvAppendArgs, FdkMeasureArgs, FdkMxfp4Args, FdkPlan
+from ._lib import FdkCombineRanksArgs, FdkDecodeArgs, FdkKvAppendArgs, FdkKvAppendAxesArgs, FdkMeasureArgs, FdkMxfp4Args, FdkPlan
 
 _LIB = _lib.load()          # raises ImportError when libfdk.so is not built - by design
 
@@ -782,7 +782,7 @@ def flash_decode_bsnh(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
     return output
 
 
-_KV_APPEND_TEMPLATES = {}      # layout key -> (validated argument block, shape of q_norm_rope, fp8 cache)
+_KV_APPEND_TEMPLATES = {}      # layout key -> (validated argument block, shape of q_norm_rope, fp8 cache, block of fdk_kv_append_axes)
 
 
 def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -790,16 +790,24 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
                                 k_rms_weight: torch.Tensor, cos_cache: torch.Tensor, sin_cache: torch.Tensor,
                                 q_norm_rope: Optional[torch.Tensor] = None, q_rms_eps: float = 1e-6,
                                 k_rms_eps: float = 1e-6, *, k_scale: Optional[torch.Tensor] = None,
-                                v_scale: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+                                v_scale: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                                rope_sections: Optional[Sequence[int]] = None, rope_interleaved: bool = False,
+                                stream=None) -> torch.Tensor:
     """The step before the decode: per-head RMSNorm and rotary embedding of the new tokens' q and k rows, and the
     append of their K / V rows to the paged cache.  Argument order of the reference's
     ``ModelBuilder.make_qk_norm_rope_update_kvcache`` (mega_triton_kernel/models/model_builder.py:341-345).
 
     qkv          [B, T, Hq + 2 Hkv, D] bf16/fp16: q heads, k heads, v heads of the T new tokens
-    key_cache    [num_pages, P, Hkv, D] in qkv's dtype or float8_e4m3fn (then with k_scale / v_scale [Hkv] fp32);
-    value_cache  updated in place at positions ``kv_lens[b] - T + t``
+    key_cache    [num_pages, P, Hkv, D] in qkv's dtype or float8_e4m3fn (then with k_scale / v_scale [Hkv] fp32), or MXFP4
+    value_cache  codes [num_pages, P, Hkv, D/2] with block scales k_scale / v_scale [num_pages, P, Hkv, D/32], which are
+                 written, too (see ``mxfp4_quantize``); updated in place at places ``kv_lens[b] - T + t``
     block_tables [B, max_pages] int32;  kv_lens [B] int32, ALREADY counting the new tokens (model_builder.py:347)
     q/k_rms_weight [D] in qkv's dtype;  cos_cache / sin_cache [S, D], [1, S, D] or [B, S, D] fp32, row = position
+    positions    int32 [B, T] or [A, B, T], A <= 4 axes (time, height, width ...): the rows of the cos / sin tables that turn
+                 the tokens' rotary pairs (clamped to the tables); default: the tokens' places in the cache
+    rope_sections  how many of the D/2 pairs each axis turns (they add up to D/2): the first ``rope_sections[0]`` pairs by
+                 axis 0 and so on; ``rope_interleaved``: pair i by axis i mod A while i // A < rope_sections[that axis], by
+                 axis 0 otherwise
     Returns ``q_norm_rope [B, T, Hq, D]`` - the query the decode takes (reshape to [B, Hq, D] for T = 1)."""
     # A decode loop calls this once per layer and step with the same layouts: the checks and the argument block depend
     # on shapes, strides, dtypes and devices only, so a call whose layouts were seen before copies the validated block
@@ -808,7 +816,7 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
         return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
     key = (meta(qkv), meta(key_cache), meta(value_cache), meta(block_tables), meta(kv_lens), meta(q_rms_weight),
            meta(k_rms_weight), meta(cos_cache), meta(sin_cache), meta(q_norm_rope), meta(k_scale), meta(v_scale),
-           q_rms_eps, k_rms_eps)
+           q_rms_eps, k_rms_eps, meta(positions), rope_sections if rope_sections is None else tuple(rope_sections), rope_interleaved)
     hit = _KV_APPEND_TEMPLATES.get(key)
     if hit is not None:
         a = FdkKvAppendArgs.from_buffer_copy(hit[0])
@@ -821,20 +829,31 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
         a.k_cache, a.v_cache = key_cache.data_ptr(), value_cache.data_ptr()
         if k_scale is not None and v_scale is not None and hit[2]:
             a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        _lib.check(_LIB.fdk_kv_append(C.byref(a), _stream_handle(stream)))
+        if hit[3] is None:
+            _lib.check(_LIB.fdk_kv_append(C.byref(a), _stream_handle(stream)))
+            return q_norm_rope
+        x = FdkKvAppendAxesArgs.from_buffer_copy(hit[3])
+        x.append = C.addressof(a)
+        if positions is not None:
+            x.positions = positions.data_ptr()
+        if a.kv_dtype == _lib.FDK_MXFP4:
+            x.k_block_scale, x.v_block_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        _lib.check(_LIB.fdk_kv_append_axes(C.byref(x), _stream_handle(stream)))
         return q_norm_rope
     q_given = q_norm_rope is not None
     if qkv.dim() != 4 or key_cache.dim() != 4 or value_cache.dim() != 4:
         raise ValueError("qkv must be [B, T, heads, D]; caches [num_pages, P, Hkv, D]")
     batch, new_tokens, heads, d = qkv.shape
-    num_pages, page_size, kv_heads, dk = key_cache.shape
+    num_pages, page_size, kv_heads, _ = key_cache.shape
+    dk = _row_values(key_cache)
     if dk != d or tuple(value_cache.shape) != tuple(key_cache.shape) or key_cache.dtype != value_cache.dtype:
         raise ValueError("caches must share shape and dtype, with qkv's head_dim")
     q_heads = heads - 2 * kv_heads
     if q_heads < 0:
         raise ValueError(f"qkv has {heads} heads, fewer than 2 * {kv_heads} kv heads")
     fp8 = key_cache.dtype == torch.float8_e4m3fn
-    if not fp8 and key_cache.dtype != qkv.dtype:
+    mx = key_cache.dtype in _MXFP4_CODES
+    if not fp8 and not mx and key_cache.dtype != qkv.dtype:
         raise ValueError("a 16-bit cache must have qkv's dtype")
     if fp8 and (k_scale is None or v_scale is None):
         raise ValueError("k_scale / v_scale are required for an fp8 cache")
@@ -856,6 +875,22 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
             block_tables.shape[0] != batch or block_tables.stride(-1) != 1 or tuple(kv_lens.shape) != (batch,) or \
             not kv_lens.is_contiguous() or not block_tables.is_cuda or not kv_lens.is_cuda:
         raise ValueError("block_tables [B, max_pages] and kv_lens [B] must be contiguous int32 GPU tensors")
+    if mx:
+        _check_block_scales("k_scale", k_scale, key_cache)
+        _check_block_scales("v_scale", v_scale, value_cache)
+    axes = 0
+    if positions is not None:
+        pos = positions if positions.dim() == 3 else positions[None]
+        if pos.dim() != 3 or tuple(pos.shape[1:]) != (batch, new_tokens) or not 1 <= pos.shape[0] <= 4 or pos.dtype != torch.int32:
+            raise ValueError(f"positions must be int32 [{batch}, {new_tokens}] or [axes, {batch}, {new_tokens}] with 1 to 4 axes")
+        if pos.device != qkv.device:
+            raise ValueError(f"positions is on {pos.device}, qkv on {qkv.device}")
+        axes = pos.shape[0]
+        sections = (d // 2,) if rope_sections is None and axes == 1 else tuple(rope_sections or ())
+        if len(sections) != axes or any(n < 0 for n in sections) or sum(sections) != d // 2:
+            raise ValueError(f"rope_sections must name the pairs of each of {axes} axes, {d // 2} in all; got {rope_sections}")
+    elif rope_sections is not None or rope_interleaved:
+        raise ValueError("rope_sections / rope_interleaved need positions")
     if q_norm_rope is None:
         q_norm_rope = torch.empty((batch, new_tokens, q_heads, d), dtype=qkv.dtype, device=qkv.device)
     elif tuple(q_norm_rope.shape) != (batch, new_tokens, q_heads, d) or q_norm_rope.dtype != qkv.dtype or \
@@ -885,12 +920,28 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
         a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
     a.q_out = q_norm_rope.data_ptr()
     a.q_out_stride_b, a.q_out_stride_t, a.q_out_stride_h = q_norm_rope.stride(0), q_norm_rope.stride(1), q_norm_rope.stride(2)
-    _lib.check(_LIB.fdk_kv_append(C.byref(a), _stream_handle(stream)))
+    x = None
+    if mx or axes:
+        x = FdkKvAppendAxesArgs()
+        x.struct_size = C.sizeof(FdkKvAppendAxesArgs)
+        x.append = C.addressof(a)
+        if mx:
+            x.k_block_scale, x.v_block_scale = k_scale.data_ptr(), v_scale.data_ptr()
+            x.kbs_stride_page, x.kbs_stride_tok, x.kbs_stride_head = k_scale.stride()[:3]
+            x.vbs_stride_page, x.vbs_stride_tok, x.vbs_stride_head = v_scale.stride()[:3]
+        if axes:
+            x.positions = pos.data_ptr()
+            x.pos_stride_axis, x.pos_stride_b, x.pos_stride_t = pos.stride()
+            x.num_axes, x.rope_interleaved = axes, int(bool(rope_interleaved))
+            x.rope_sections = (C.c_int32 * 4)(*sections)
+        _lib.check(_LIB.fdk_kv_append_axes(C.byref(x), _stream_handle(stream)))
+    else:
+        _lib.check(_LIB.fdk_kv_append(C.byref(a), _stream_handle(stream)))
     # (only after the library has accepted the block; a result tensor of the call's own has the contiguous layout)
     if q_given or q_norm_rope.is_contiguous():
         if len(_KV_APPEND_TEMPLATES) >= 256:
             _KV_APPEND_TEMPLATES.clear()
-        _KV_APPEND_TEMPLATES[key] = (bytes(a), tuple(q_norm_rope.shape), fp8)
+        _KV_APPEND_TEMPLATES[key] = (bytes(a), tuple(q_norm_rope.shape), fp8, None if x is None else bytes(x))
     return q_norm_rope
 
 
