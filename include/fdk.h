@@ -344,6 +344,72 @@ typedef struct fdk_mxfp4_args {
     int32_t reserved;
 } fdk_mxfp4_args;
 
+/* (revision 3) Attention weights per cached token, for the eviction of those that receive little:
+ *   weights[b, kvh, n] += sum over the q heads h of kv head kvh of exp(logit(b, h, n) - lse[b, h]),  n < kv_lens[b],
+ * logit being the scaled (and soft-capped) logit of the decode and lse what it returned.  K rows of 64, 128, 192, 256 or 576
+ * values (MXFP4: 64, 128, 256).  Lengths are clamped to weights_len and to the table.  Nothing else is written. */
+typedef struct fdk_attn_weights_args {
+    uint32_t struct_size;
+    uint32_t flags;       /* FDK_FLAG_DRY_RUN */
+    const void* q;        /* [B, Hq, D] */
+    int64_t q_stride_b, q_stride_h;
+    int32_t q_dtype;      /* FDK_BF16 | FDK_FP16 */
+    int32_t kv_dtype;     /* q_dtype | FDK_FP8_E4M3 | FDK_MXFP4 */
+    const void* k_cache;  /* [num_pages, P, Hkv, D] */
+    int64_t k_stride_page, k_stride_tok, k_stride_head;
+    const float* k_scale; /* [Hkv], fp8 caches only (null = 1.0) */
+    const uint8_t* k_block_scale; /* MXFP4 caches: [num_pages, P, Hkv, D/32], byte strides */
+    int64_t kbs_stride_page, kbs_stride_tok, kbs_stride_head;
+    const int32_t* block_table; /* [B, max_pages] */
+    int64_t table_stride_b;
+    const int32_t* kv_lens;     /* [B] */
+    const float* lse;           /* [B, Hq] */
+    int64_t lse_stride_b;
+    float* weights;             /* [B, Hkv, weights_len], updated in place */
+    int64_t weights_stride_b, weights_stride_h;
+    int32_t batch, num_q_heads, num_kv_heads, head_dim;
+    int32_t page_size, max_pages, weights_len;
+    float sm_scale, soft_cap;   /* soft_cap <= 0: off */
+    int32_t reserved;
+} fdk_attn_weights_args;
+
+/* (revision 3) Eviction.  Of a sequence's n = kv_lens[b] tokens (clamped to weights_len and to the table) the last `recent`
+ * stay and, of the others, those with the largest weights - ties: the lowest slots; a NaN counts as the largest -, `keep` in
+ * all; every kv head chooses for itself.  The survivors' rows move to slots 0 .. in their order, in place; rows behind the new
+ * length keep their contents, pages of the table keep their owners.  A sequence of at most `keep` tokens stays as it is.
+ *   kept[b, kvh, j]  the slot that the token in slot j had before, -1 behind the new length
+ *   weights_out      the survivors' weights, 0 behind them; may be `weights` itself (same strides), no other overlap
+ *   kv_lens_out      min(n, keep); may be `kv_lens` itself */
+typedef struct fdk_kv_evict_args {
+    uint32_t struct_size;
+    uint32_t flags;       /* FDK_FLAG_DRY_RUN */
+    int32_t kv_dtype;     /* FDK_BF16 | FDK_FP16 | FDK_FP8_E4M3 | FDK_MXFP4 */
+    int32_t reserved0;
+    void* k_cache;        /* [num_pages, P, Hkv, D], rows of a multiple of 16 bytes */
+    void* v_cache;        /* [num_pages, P, Hkv, Dv] */
+    int64_t k_stride_page, k_stride_tok, k_stride_head;
+    int64_t v_stride_page, v_stride_tok, v_stride_head;
+    uint8_t* k_block_scale; /* MXFP4 caches: the scales move with the rows; byte strides */
+    uint8_t* v_block_scale;
+    int64_t kbs_stride_page, kbs_stride_tok, kbs_stride_head;
+    int64_t vbs_stride_page, vbs_stride_tok, vbs_stride_head;
+    const int32_t* block_table; /* [B, max_pages] */
+    int64_t table_stride_b;
+    const int32_t* kv_lens;     /* [B] */
+    const float* weights;       /* [B, Hkv, weights_len] */
+    int64_t weights_stride_b, weights_stride_h;
+    float* weights_out;         /* [B, Hkv, weights_len] */
+    int64_t weights_out_stride_b, weights_out_stride_h;
+    int32_t* kept;              /* [B, Hkv, keep], contiguous */
+    int32_t* kv_lens_out;       /* [B] */
+    void* workspace;            /* fdk_kv_evict_workspace_bytes, 16-byte aligned; contents unspecified before and after */
+    size_t workspace_bytes;
+    int32_t batch, num_kv_heads, head_dim, v_head_dim; /* v_head_dim 0: head_dim */
+    int32_t page_size, max_pages, weights_len;
+    int32_t keep, recent;       /* 0 <= recent <= keep, 1 <= keep <= weights_len */
+    int32_t reserved1;
+} fdk_kv_evict_args;
+
 struct fdk_measure_args; /* include/fdk_measure.h */
 
 int fdk_abi_version(void);
@@ -412,6 +478,13 @@ int fdk_kv_append(const fdk_kv_append_args* args, void* hip_stream);
 
 /* ... with explicit positions, or into an MXFP4 cache (see fdk_kv_append_axes_args). */
 int fdk_kv_append_axes(const fdk_kv_append_axes_args* args, void* hip_stream);
+
+/* Add the attention weights of one query token per sequence to the cached tokens' sums (see fdk_attn_weights_args). */
+int fdk_accumulate_weights(const fdk_attn_weights_args* args, void* hip_stream);
+
+/* Evict the tokens of least weight (see fdk_kv_evict_args).  Calls that overlap in time need distinct workspaces. */
+int fdk_kv_evict(const fdk_kv_evict_args* args, void* hip_stream);
+size_t fdk_kv_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads);
 
 #ifdef __cplusplus
 }

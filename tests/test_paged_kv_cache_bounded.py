@@ -1,0 +1,122 @@
+"""A paged cache in 4 bits, kept at a budget: bookkeeping on the CPU, and a serving loop - append with positions of three
+axes, decode, attention weights, eviction - against 64 bits on the GPU."""
+import pytest
+import torch
+
+from oracle import kv_evict as okv
+from oracle import mxfp4, rope_axes
+from triton_distributed_amd.paged_kv_cache import PagedKVCache
+
+
+def _cache(device, dtype=torch.float4_e2m1fn_x2, layers=2, batch=3, **kw):
+    return PagedKVCache(PAGE_SIZE=4, num_layers=layers, batch_size=batch, max_length=64, num_kv_heads=2, head_dim=64, dtype=dtype,
+                        device=device, generator=torch.Generator().manual_seed(1), **kw)
+
+
+def test_mxfp4_pools():
+    c = _cache("cpu")
+    blocks = 16 * 3 * 2
+    assert tuple(c.key_cache.shape) == (blocks, 4, 2, 32) == tuple(c.value_cache.shape)
+    assert c.key_cache.dtype == torch.float4_e2m1fn_x2
+    assert tuple(c.k_block_scale.shape) == (blocks, 4, 2, 2) == tuple(c.v_block_scale.shape)
+    assert c.nbytes == 2 * blocks * 4 * 2 * 34
+    assert c.layer_scales(1) == (c.k_block_scale, c.v_block_scale)
+    assert not c.key_cache.view(torch.uint8).any() and (c.value_cache.data_ptr() - c.key_cache.data_ptr()) % 512 == 256
+    with pytest.raises(ValueError, match="zeroed"):
+        _cache("cpu", fill="randn")
+    with pytest.raises(ValueError, match="multiple of 32"):
+        PagedKVCache(head_dim=48, max_length=8, num_layers=1, dtype=torch.float4_e2m1fn_x2, device="cpu")
+
+
+def test_positions_and_refusals_without_a_gpu():
+    c = _cache("cpu")
+    c.inc_offset(5)
+    c.inc_offset(2)
+    assert c.next_positions(2).tolist() == [[5, 6]] * 3 and c.next_positions(2).dtype == torch.int32
+    w = torch.zeros(2, 3, 2, 7)
+    assert c.evict(w, 7, 2) is None and c.max_kv_len == 7                  # nothing has to go
+    for bad in (w[0], w[:1], w[..., :6]):
+        with pytest.raises(ValueError, match="weights"):
+            c.evict(bad, 3, 1)
+    with pytest.raises(ValueError, match="GPU"):
+        c.evict(w, 3, 1)
+    assert c.max_kv_len == 7 and c.next_positions(1).tolist() == [[6]] * 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float4_e2m1fn_x2, torch.bfloat16])
+def test_a_serving_loop_at_a_budget(cuda_device, dtype):
+    """Prompt, then single tokens; after every decode the weights, an eviction whenever the budget is exceeded by four
+    tokens.  Every step's decode, weights, survivors and rows against the oracle, which carries its own copy of the cache."""
+    dev, b, hq, hkv, d, layers, keep, recent = cuda_device, 3, 4, 2, 64, 2, 20, 6
+    c = _cache(dev, dtype)
+    g = torch.Generator().manual_seed(2)
+    sections, scale = (12, 10, 10), 0.125
+    ang = torch.rand(200, d // 2, generator=g) * 6.28
+    cos, sin = ang.cos(), ang.sin()
+    wq, wk = ((1 + 0.1 * torch.randn(d, generator=g)).bfloat16() for _ in range(2))
+    S = 40
+    weights = torch.zeros(layers, b, hkv, S, device=dev)
+    seen, evictions = 0, 0
+    tables = c.block_tables.cpu()
+
+    def values():
+        """K and V of the pools in 64 bits."""
+        if c.mxfp4:
+            return [mxfp4.dequantize(x, s) for x, s in ((c.key_cache, c.k_block_scale), (c.value_cache, c.v_block_scale))]
+        return [x.cpu().double() for x in (c.key_cache, c.value_cache)]
+
+    for step in range(14):
+        new = 17 if step == 0 else 1
+        c.inc_offset(new)
+        lens = [c.max_kv_len] * b
+        time = torch.arange(seen, seen + new, dtype=torch.int32).expand(b, new)
+        assert torch.equal(c.next_positions(new).cpu(), time)
+        positions = torch.stack((time, time // 3 + 1, time % 5))
+        seen += new
+        for layer in range(layers):
+            qkv = torch.randn(b, new, hq + 2 * hkv, d, generator=g).bfloat16()
+            before = values()
+            q = c.append(layer, qkv.to(dev), wq.to(dev), wk.to(dev), cos.to(dev), sin.to(dev), positions=positions.to(dev),
+                         rope_sections=sections)
+            want, pair = rope_axes.norm_rope(qkv[:, :, :hq], wq, 1e-6, cos, sin, positions, sections, False)
+            assert ((q.cpu().double() - want).abs() <= 2.0 ** -7 * (pair + want.abs()) + 2.0 ** -20).all()
+            after = values()
+            v16 = qkv[:, :, hq + hkv:]
+            v_want = mxfp4.dequantize(*mxfp4.quantize(v16)) if c.mxfp4 else v16.double()
+            for i in range(b):
+                for t in range(new):
+                    at = lens[i] - new + t
+                    pg, slot = int(tables[layer, i, at // 4]), at % 4
+                    assert torch.equal(after[1][pg, slot], v_want[i, t])
+                    before[1][pg, slot] = v_want[i, t]
+            assert torch.equal(after[1], before[1])                       # nothing else moved
+            q1 = q[:, -1].contiguous()
+            out, lse = c.decode(layer, q1, scale)
+            o64, l64, spread = mxfp4.decode(q1, after[0], after[1], tables[layer], lens, scale)
+            assert ((out.cpu().double() - o64).abs() <= 2.0 ** -8 * (spread + o64.abs()) + 2.0 ** -12 * spread + 2.0 ** -20).all()
+            torch.testing.assert_close(lse.cpu().double(), l64, atol=2.0 ** -14, rtol=2.0 ** -20)
+            w_before = weights[layer].cpu().double()
+            c.accumulate(layer, q1, lse, scale, weights[layer])
+            add, _ = okv.token_weights(q1, after[0], tables[layer], lens, lse, scale, length=S)
+            torch.testing.assert_close(weights[layer].cpu().double(), w_before + add, rtol=2.0 ** -12, atol=2.0 ** -20)
+        if c.max_kv_len >= keep + 4:
+            pools = [x.cpu().view(torch.uint8) if x is not None else None for x in (c.key_cache, c.value_cache, c.k_block_scale, c.v_block_scale)]
+            pools = [x for x in pools if x is not None]
+            w_before = weights.cpu()
+            kept = c.evict(weights, keep, recent)
+            for layer in range(layers):
+                pools, new_lens, want_kept, want_w = okv.evict(pools, tables[layer], lens, w_before[layer], keep, recent)
+                assert torch.equal(kept[layer].cpu(), want_kept) and torch.equal(weights[layer].cpu(), want_w)
+            assert torch.equal(c.kv_lens.cpu(), new_lens) and c.max_kv_len == keep
+            got = [x.cpu().view(torch.uint8) for x in (c.key_cache, c.value_cache, c.k_block_scale, c.v_block_scale) if x is not None]
+            assert all(torch.equal(a, w) for a, w in zip(got, pools))
+            evictions += 1
+    assert evictions >= 2
+    # one more token, at the position that follows all that were seen
+    c.inc_offset(1)
+    assert c.next_positions(1).tolist() == [[seen]] * b
+    qkv = torch.randn(b, 1, hq + 2 * hkv, d, generator=g).bfloat16()
+    q = c.append(0, qkv.to(dev), wq.to(dev), wk.to(dev), cos.to(dev), sin.to(dev))
+    want, pair = rope_axes.norm_rope(qkv[:, :, :hq], wq, 1e-6, cos, sin, torch.full((1, b, 1), seen), (d // 2,), False)
+    assert ((q.cpu().double() - want).abs() <= 2.0 ** -7 * (pair + want.abs()) + 2.0 ** -20).all()

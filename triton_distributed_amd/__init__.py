@@ -8,7 +8,7 @@ imports without the library.
 import importlib
 
 __all__ = [
-    "LengthFeedback", "PreparedDecode", "SplitKvPlan", "flash_decode", "flash_decode_bsnh", "get_split_kv_plan", "gqa_fwd_batch_decode",
+    "accumulate_attention_weights", "evict_kvcache", "LengthFeedback", "PreparedDecode", "SplitKvPlan", "flash_decode", "flash_decode_bsnh", "get_split_kv_plan", "gqa_fwd_batch_decode",
     "gqa_fwd_batch_decode_aot", "gqa_fwd_batch_decode_intra_rank", "gqa_fwd_batch_decode_intra_rank_aot",
     "gqa_fwd_batch_decode_persistent", "gqa_fwd_batch_decode_persistent_aot",
     "inter_rank_combine", "mxfp4_dequantize", "mxfp4_quantize", "pack_out_lse", "prepare_decode", "probe_linear_read", "qk_norm_rope_update_kvcache",
@@ -23,8 +23,8 @@ _HOST_ONLY = {"PagedKVCache": ".paged_kv_cache", "alloc_kv_pools": ".paged_kv_ca
 def _bind():
     """Import the entry points (loads libfdk.so; raises if it is missing) and bind them on the package: the
     function ``flash_decode`` takes the place of the submodule attribute of the same name that the import sets."""
-    mod = importlib.import_module(".flash_decode", __name__)
-    globals().update({n: getattr(mod, n) for n in __all__})
+    mods = [importlib.import_module(m, __name__) for m in (".flash_decode", ".kv_evict")]
+    globals().update({n: getattr(next(m for m in mods if hasattr(m, n)), n) for n in __all__})
 
 
 def __getattr__(name):

@@ -29,7 +29,7 @@ EXPORTS = (
     "fdk_abi_version", "fdk_abi_revision", "fdk_last_error", "fdk_device_cus", "fdk_plan", "fdk_workspace_bytes",
     "fdk_decode", "fdk_decode_splitkv", "fdk_combine", "fdk_combine_ranks", "fdk_counters_len", "fdk_kv_append",
     "fdk_decode_static", "fdk_length_feedback_alloc", "fdk_length_feedback_free", "fdk_mx_quantize", "fdk_mx_dequantize",
-    "fdk_kv_append_axes",
+    "fdk_kv_append_axes", "fdk_accumulate_weights", "fdk_kv_evict", "fdk_kv_evict_workspace_bytes",
 )
 # declared in include/fdk_measure.h
 MEASURE_EXPORTS = ("fdk_probe_linear_read",)
@@ -134,6 +134,41 @@ class FdkMxfp4Args(C.Structure):
     ]
 
 
+class FdkAttnWeightsArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("flags", C.c_uint32),
+        ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_h", C.c_int64), ("q_dtype", C.c_int32), ("kv_dtype", C.c_int32),
+        ("k_cache", C.c_void_p), ("k_stride_page", C.c_int64), ("k_stride_tok", C.c_int64), ("k_stride_head", C.c_int64),
+        ("k_scale", C.c_void_p), ("k_block_scale", C.c_void_p),
+        ("kbs_stride_page", C.c_int64), ("kbs_stride_tok", C.c_int64), ("kbs_stride_head", C.c_int64),
+        ("block_table", C.c_void_p), ("table_stride_b", C.c_int64), ("kv_lens", C.c_void_p),
+        ("lse", C.c_void_p), ("lse_stride_b", C.c_int64),
+        ("weights", C.c_void_p), ("weights_stride_b", C.c_int64), ("weights_stride_h", C.c_int64),
+        ("batch", C.c_int32), ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("max_pages", C.c_int32), ("weights_len", C.c_int32),
+        ("sm_scale", C.c_float), ("soft_cap", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
+class FdkKvEvictArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("flags", C.c_uint32), ("kv_dtype", C.c_int32), ("reserved0", C.c_int32),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("k_stride_page", C.c_int64), ("k_stride_tok", C.c_int64), ("k_stride_head", C.c_int64),
+        ("v_stride_page", C.c_int64), ("v_stride_tok", C.c_int64), ("v_stride_head", C.c_int64),
+        ("k_block_scale", C.c_void_p), ("v_block_scale", C.c_void_p),
+        ("kbs_stride_page", C.c_int64), ("kbs_stride_tok", C.c_int64), ("kbs_stride_head", C.c_int64),
+        ("vbs_stride_page", C.c_int64), ("vbs_stride_tok", C.c_int64), ("vbs_stride_head", C.c_int64),
+        ("block_table", C.c_void_p), ("table_stride_b", C.c_int64), ("kv_lens", C.c_void_p),
+        ("weights", C.c_void_p), ("weights_stride_b", C.c_int64), ("weights_stride_h", C.c_int64),
+        ("weights_out", C.c_void_p), ("weights_out_stride_b", C.c_int64), ("weights_out_stride_h", C.c_int64),
+        ("kept", C.c_void_p), ("kv_lens_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("batch", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("v_head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("max_pages", C.c_int32), ("weights_len", C.c_int32),
+        ("keep", C.c_int32), ("recent", C.c_int32), ("reserved1", C.c_int32),
+    ]
+
+
 class FdkError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"fdk error {code}: {message}")
@@ -188,6 +223,12 @@ def load() -> C.CDLL:
     lib.fdk_kv_append.argtypes = [C.POINTER(FdkKvAppendArgs), C.c_void_p]
     lib.fdk_kv_append_axes.restype = C.c_int
     lib.fdk_kv_append_axes.argtypes = [C.POINTER(FdkKvAppendAxesArgs), C.c_void_p]
+    lib.fdk_accumulate_weights.restype = C.c_int
+    lib.fdk_accumulate_weights.argtypes = [C.POINTER(FdkAttnWeightsArgs), C.c_void_p]
+    lib.fdk_kv_evict.restype = C.c_int
+    lib.fdk_kv_evict.argtypes = [C.POINTER(FdkKvEvictArgs), C.c_void_p]
+    lib.fdk_kv_evict_workspace_bytes.restype = C.c_size_t
+    lib.fdk_kv_evict_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
     for name in ("fdk_mx_quantize", "fdk_mx_dequantize"):
         fn = getattr(lib, name)
         fn.restype = C.c_int

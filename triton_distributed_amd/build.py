@@ -39,6 +39,8 @@ SOURCES = [
     "fdk_splitkv_mfma_d576v512_shared.hip", "fdk_splitkv_mfma_d576v512_shared_queue.hip", "fdk_splitkv_mfma_d576v512_shared_bal.hip",
     # rows of 128 values with more than 16 q heads per kv head
     "fdk_splitkv_mfma_d128_tiled.hip", "fdk_splitkv_mfma_d128_tiled_queue.hip", "fdk_splitkv_mfma_d128_tiled_bal.hip",
+    # attention weights per cached token, eviction
+    "fdk_attn_weights.hip", "fdk_kv_evict.hip",
     # MXFP4 caches; appends with explicit positions
     "fdk_kv_append_axes.hip", "fdk_mxfp4.hip", "fdk_splitkv_mx4_d64.hip", "fdk_splitkv_mx4_d128.hip", "fdk_splitkv_mx4_d256.hip",
 ]

@@ -11,6 +11,7 @@
 
 #include "../../include/fdk_measure.h"
 #include "fdk_device.h"
+#include "fdk_kv_evict.h"
 #include "fdk_mxfp4.h"
 
 namespace {
@@ -990,6 +991,163 @@ int fdk_kv_append_axes(const fdk_kv_append_axes_args* args, void* hip_stream) {
     fdk_kv_append_axes_args local;
     if (int rc = adopt(args, args->struct_size, sizeof(fdk_kv_append_axes_args), "fdk_kv_append_axes_args", &local)) return rc;
     return kv_append(local.append, &local, hip_stream);
+}
+
+// what the two calls below check of a paged cache; strides in elements of `es` bytes
+static int check_pages(int batch, int page_size, int max_pages, int64_t table_stride_b, const void* table, const void* kv_lens) {
+    if (page_size <= 0 || max_pages <= 0) return fail(FDK_ESHAPE, "page_size %d, max_pages %d must be positive", page_size, max_pages);
+    if ((int64_t)max_pages * page_size > kMaxTableTokens)
+        return fail(FDK_ESHAPE, "max_pages*page_size = %lld: a block_table row may address at most 2^30 tokens",
+                    (long long)((int64_t)max_pages * page_size));
+    if (batch > 65535) return fail(FDK_ESHAPE, "at most 65535 sequences");
+    if (!table || !kv_lens) return fail(FDK_ENULL, "block_table / kv_lens must be non-null");
+    if ((reinterpret_cast<uintptr_t>(table) & 3u) || (reinterpret_cast<uintptr_t>(kv_lens) & 3u))
+        return fail(FDK_EALIGN, "block_table / kv_lens must be 4-byte aligned");
+    if (table_stride_b < max_pages) return fail(FDK_ESHAPE, "table_stride_b %lld < max_pages %d", (long long)table_stride_b, max_pages);
+    return FDK_OK;
+}
+
+static int check_rows(const char* what, const void* cache, int64_t sp, int64_t st, int64_t sh, int es, int row_bytes, int num_kv_heads) {
+    if (!cache) return fail(FDK_ENULL, "%s must be non-null", what);
+    if (!aligned16(cache)) return fail(FDK_EALIGN, "%s must be 16-byte aligned", what);
+    if (sp < 0 || st < 0 || sh < 0) return fail(FDK_ESHAPE, "negative %s stride", what);
+    if ((sp * es) % 16 || (st * es) % 16 || (num_kv_heads > 1 && (sh * es) % 16))
+        return fail(FDK_EALIGN, "%s strides must be multiples of 16 bytes", what);
+    if (num_kv_heads > 1 && sh * es < row_bytes) return fail(FDK_ESHAPE, "%s head stride shorter than a row", what);
+    return FDK_OK;
+}
+
+int fdk_accumulate_weights(const fdk_attn_weights_args* caller_args, void* hip_stream) {
+    g_err[0] = 0;
+    if (!caller_args) return fail(FDK_ENULL, "args is null");
+    fdk_attn_weights_args local;
+    if (int rc = adopt(caller_args, caller_args->struct_size, sizeof(fdk_attn_weights_args), "fdk_attn_weights_args", &local)) return rc;
+    const fdk_attn_weights_args* a = &local;
+    if (a->batch < 0) return fail(FDK_ESHAPE, "batch %d < 0", a->batch);
+    if (a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->num_q_heads % a->num_kv_heads)
+        return fail(FDK_ESHAPE, "bad head counts Hq=%d Hkv=%d", a->num_q_heads, a->num_kv_heads);
+    if (a->q_dtype != FDK_BF16 && a->q_dtype != FDK_FP16) return fail(FDK_EUNSUPPORTED, "q_dtype %d (bf16 or fp16 only)", a->q_dtype);
+    const bool mx = a->kv_dtype == FDK_MXFP4;
+    if (a->kv_dtype != a->q_dtype && a->kv_dtype != FDK_FP8_E4M3 && !mx)
+        return fail(FDK_EUNSUPPORTED, "kv_dtype %d must equal q_dtype or be fp8_e4m3 or mxfp4", a->kv_dtype);
+    const int d = a->head_dim;
+    if (d != 64 && d != 128 && d != 256 && (mx || (d != 192 && d != 576)))
+        return fail(FDK_EUNSUPPORTED, "head_dim %d not built (64, 128, 256; 16-bit and fp8 caches also 192, 576)", d);
+    if (!(fabsf(a->sm_scale) <= FLT_MAX)) return fail(FDK_ESHAPE, "sm_scale is not finite");
+    if (!(a->soft_cap <= FLT_MAX)) return fail(FDK_ESHAPE, "soft_cap is not a finite number (<= 0 switches it off)");
+    if (a->weights_len <= 0) return fail(FDK_ESHAPE, "weights_len %d <= 0", a->weights_len);
+    if (a->batch == 0) return FDK_OK;
+    if (int rc = check_pages(a->batch, a->page_size, a->max_pages, a->table_stride_b, a->block_table, a->kv_lens)) return rc;
+    const int es = elem_size(a->kv_dtype), row_bytes = mx ? d / 2 : d * es;
+    if (int rc = check_rows("k_cache", a->k_cache, a->k_stride_page, a->k_stride_tok, a->k_stride_head, es, row_bytes, a->num_kv_heads)) return rc;
+    if (!a->q || !a->lse || !a->weights) return fail(FDK_ENULL, "q / lse / weights must be non-null");
+    if (!aligned16(a->q) || a->q_stride_b % 8 || a->q_stride_h % 8) return fail(FDK_EALIGN, "q and its strides must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(a->lse) | reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->k_scale)) & 3u)
+        return fail(FDK_EALIGN, "lse / weights / k_scale must be 4-byte aligned");
+    if (a->lse_stride_b < a->num_q_heads) return fail(FDK_ESHAPE, "lse_stride_b %lld < Hq", (long long)a->lse_stride_b);
+    // (every weight is one wavefront's: rows must not overlap)
+    if ((a->num_kv_heads > 1 && a->weights_stride_h < a->weights_len) || (a->batch > 1 && a->weights_stride_b < a->weights_len))
+        return fail(FDK_ESHAPE, "weights rows overlap");
+    if (mx) {
+        if (!a->k_block_scale) return fail(FDK_ENULL, "k_block_scale is required for an mxfp4 cache");
+        if (int rc = check_scale_strides(a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head, d, a->num_kv_heads, a->page_size)) return rc;
+    }
+    const bool dry = (a->flags & FDK_FLAG_DRY_RUN) != 0;
+    const int cus = dry ? kDryRunCus : query_cus();
+    if ((int64_t)a->batch * a->num_kv_heads > INT32_MAX / 2 - 8 * (int64_t)cus) return fail(FDK_ESHAPE, "grid too large");
+    if (dry) return FDK_OK;
+    fdk::AttnWeightsParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = a->q; p.k = a->k_cache; p.k_block_scale = mx ? a->k_block_scale : nullptr;
+    p.k_scale = a->kv_dtype == FDK_FP8_E4M3 ? a->k_scale : nullptr;
+    p.block_table = a->block_table; p.kv_lens = a->kv_lens; p.lse = a->lse; p.weights = a->weights;
+    p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h;
+    p.k_sp = a->k_stride_page * es; p.k_st = a->k_stride_tok * es; p.k_sh = a->k_stride_head * es;
+    p.bs_sp = a->kbs_stride_page; p.bs_st = a->kbs_stride_tok; p.bs_sh = a->kbs_stride_head;
+    p.tbl_sb = a->table_stride_b; p.lse_sb = a->lse_stride_b; p.w_sb = a->weights_stride_b; p.w_sh = a->weights_stride_h;
+    p.batch = a->batch; p.hkv = a->num_kv_heads; p.group = a->num_q_heads / a->num_kv_heads;
+    p.page_size = a->page_size; p.page_shift = ilog2_exact(a->page_size);
+    p.max_tokens = a->max_pages * a->page_size;
+    if (p.max_tokens > a->weights_len) p.max_tokens = a->weights_len;
+    p.scale_log2 = a->sm_scale * fdk::kLog2e; p.sm_scale = a->sm_scale; p.soft_cap = a->soft_cap > 0.f ? a->soft_cap : 0.f;
+    const int rc = fdk::launch_attn_weights(p, d, a->q_dtype, a->kv_dtype, cus, reinterpret_cast<hipStream_t>(hip_stream));
+    if (rc) return fail(rc, "attention weights launch failed: %s", hipGetErrorString((hipError_t)rc));
+    return FDK_OK;
+}
+
+size_t fdk_kv_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads) {
+    if (batch <= 0 || num_kv_heads <= 0) return 0;
+    return (size_t)batch * (size_t)num_kv_heads * 16;
+}
+
+int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
+    g_err[0] = 0;
+    if (!caller_args) return fail(FDK_ENULL, "args is null");
+    fdk_kv_evict_args local;
+    if (int rc = adopt(caller_args, caller_args->struct_size, sizeof(fdk_kv_evict_args), "fdk_kv_evict_args", &local)) return rc;
+    const fdk_kv_evict_args* a = &local;
+    const int dv = a->v_head_dim > 0 ? a->v_head_dim : a->head_dim;
+    if (a->batch < 0) return fail(FDK_ESHAPE, "batch %d < 0", a->batch);
+    if (a->num_kv_heads <= 0 || a->num_kv_heads > 65535) return fail(FDK_ESHAPE, "num_kv_heads %d outside [1, 65535]", a->num_kv_heads);
+    const bool mx = a->kv_dtype == FDK_MXFP4;
+    if (a->kv_dtype != FDK_BF16 && a->kv_dtype != FDK_FP16 && a->kv_dtype != FDK_FP8_E4M3 && !mx)
+        return fail(FDK_EUNSUPPORTED, "kv_dtype %d", a->kv_dtype);
+    const int es = elem_size(a->kv_dtype);
+    // (the row length decides how a row is cut; bounded so that slices x parts stay a grid)
+    if (a->head_dim <= 0 || dv <= 0 || a->head_dim > 4096 || dv > 4096 || a->head_dim % 32 || dv % 32)
+        return fail(FDK_EUNSUPPORTED, "head_dim %d / v_head_dim %d: multiples of 32 up to 4096", a->head_dim, dv);
+    if (a->weights_len <= 0) return fail(FDK_ESHAPE, "weights_len %d <= 0", a->weights_len);
+    if (a->keep < 1 || a->keep > a->weights_len) return fail(FDK_ESHAPE, "keep %d outside [1, weights_len = %d]", a->keep, a->weights_len);
+    if (a->recent < 0 || a->recent > a->keep) return fail(FDK_ESHAPE, "recent %d outside [0, keep = %d]", a->recent, a->keep);
+    if (a->batch == 0) return FDK_OK;
+    if (int rc = check_pages(a->batch, a->page_size, a->max_pages, a->table_stride_b, a->block_table, a->kv_lens)) return rc;
+    const int kb = mx ? a->head_dim / 2 : a->head_dim * es, vb = mx ? dv / 2 : dv * es;
+    if (int rc = check_rows("k_cache", a->k_cache, a->k_stride_page, a->k_stride_tok, a->k_stride_head, es, kb, a->num_kv_heads)) return rc;
+    if (int rc = check_rows("v_cache", a->v_cache, a->v_stride_page, a->v_stride_tok, a->v_stride_head, es, vb, a->num_kv_heads)) return rc;
+    if (mx) {
+        if (!a->k_block_scale || !a->v_block_scale)
+            return fail(FDK_ENULL, "k_block_scale / v_block_scale are required for an mxfp4 cache");
+        int rc = check_scale_strides(a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
+        if (!rc) rc = check_scale_strides(a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head, dv, a->num_kv_heads, a->page_size);
+        if (rc) return rc;
+    }
+    if (!a->weights || !a->weights_out || !a->kept || !a->kv_lens_out)
+        return fail(FDK_ENULL, "weights / weights_out / kept / kv_lens_out must be non-null");
+    if ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out) | reinterpret_cast<uintptr_t>(a->kept) |
+         reinterpret_cast<uintptr_t>(a->kv_lens_out)) & 3u)
+        return fail(FDK_EALIGN, "weights / weights_out / kept / kv_lens_out must be 4-byte aligned");
+    if ((a->num_kv_heads > 1 && a->weights_out_stride_h < a->weights_len) || (a->batch > 1 && a->weights_out_stride_b < a->weights_len))
+        return fail(FDK_ESHAPE, "weights_out rows overlap");
+    if (a->weights_stride_b < 0 || a->weights_stride_h < 0) return fail(FDK_ESHAPE, "negative weights stride");
+    if (a->weights == a->weights_out &&
+        ((a->num_kv_heads > 1 && a->weights_stride_h != a->weights_out_stride_h) || (a->batch > 1 && a->weights_stride_b != a->weights_out_stride_b)))
+        return fail(FDK_ESHAPE, "weights_out may be weights itself only with its strides");
+    const size_t need = fdk_kv_evict_workspace_bytes(a->batch, a->num_kv_heads);
+    if (!a->workspace || a->workspace_bytes < need) return fail(FDK_EWORKSPACE, "workspace has %zu bytes; %zu needed", a->workspace ? a->workspace_bytes : 0, need);
+    if (!aligned16(a->workspace)) return fail(FDK_EALIGN, "workspace must be 16-byte aligned");
+    if (a->flags & FDK_FLAG_DRY_RUN) return FDK_OK;
+    fdk::EvictParams p;
+    memset(&p, 0, sizeof(p));
+    p.num_tensors = mx ? 4 : 2;
+    p.rows[0] = fdk::EvictRows{static_cast<char*>(a->k_cache), a->k_stride_page * es, a->k_stride_tok * es, a->k_stride_head * es, kb / 16, 16};
+    p.rows[1] = fdk::EvictRows{static_cast<char*>(a->v_cache), a->v_stride_page * es, a->v_stride_tok * es, a->v_stride_head * es, vb / 16, 16};
+    if (mx) {
+        p.rows[2] = fdk::EvictRows{reinterpret_cast<char*>(a->k_block_scale), a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head,
+                                   a->head_dim / fdk::kMxBlock, 1};
+        p.rows[3] = fdk::EvictRows{reinterpret_cast<char*>(a->v_block_scale), a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head,
+                                   dv / fdk::kMxBlock, 1};
+    }
+    p.block_table = a->block_table; p.kv_lens = a->kv_lens; p.weights = a->weights; p.weights_out = a->weights_out;
+    p.kept = a->kept; p.plan = static_cast<int32_t*>(a->workspace); p.kv_lens_out = a->kv_lens_out;
+    p.tbl_sb = a->table_stride_b; p.w_sb = a->weights_stride_b; p.w_sh = a->weights_stride_h;
+    p.wo_sb = a->weights_out_stride_b; p.wo_sh = a->weights_out_stride_h;
+    p.batch = a->batch; p.hkv = a->num_kv_heads; p.keep = a->keep; p.recent = a->recent;
+    p.weights_len = a->weights_len;
+    p.max_tokens = a->max_pages * a->page_size < a->weights_len ? a->max_pages * a->page_size : a->weights_len;
+    p.page_size = a->page_size; p.page_shift = ilog2_exact(a->page_size);
+    const int rc = fdk::launch_kv_evict(p, query_cus(), reinterpret_cast<hipStream_t>(hip_stream));
+    if (rc) return fail(rc, "eviction launch failed: %s", hipGetErrorString((hipError_t)rc));
+    return FDK_OK;
 }
 
 }  // extern "C"

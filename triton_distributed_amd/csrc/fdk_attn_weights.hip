@@ -1,0 +1,236 @@
+// weights[b, kvh, n] += sum over the q heads of the group of exp(logit(b, h, n) - lse[b, h]): what each cached token receives
+// from the query's attention, given the log-sum-exp that the decode returns.  gfx950.
+//
+// One pass over the K rows, no softmax of its own: the logits of 16 tokens x 16 q heads are S = Q K^T by MFMA with both
+// operands loaded straight in their layouts, K as operand B (lane (c, a): token c, its a-th piece of every 64 bytes), so that
+// lane (c, a) holds token c's logits of heads 4a .. 4a + 3 and the sum over the heads is three additions and two exchanges.
+// Every weight belongs to one wavefront: no atomics, the same bits on every run.  A workgroup takes a share of a sequence for
+// one kv head; its wavefronts interleave steps.  Bound by the bytes of the K rows.
+#include "fdk_kv_evict.h"
+
+namespace fdk {
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+enum KeyKind { KEY_16BIT = 0, KEY_FP8 = 1, KEY_MX4 = 2 };
+
+template <int QDT>
+__device__ __forceinline__ f32x4_t mma16(uint4 a, uint4 b, f32x4_t c) {
+    if constexpr (QDT == FDK_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// (the sum over lanes l, l ^ 16, l ^ 32, l ^ 48, see max_across_rows in fdk_splitkv_mfma.h)
+__device__ __forceinline__ float sum_across_rows(float x) {
+    float a = x, b = x;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    a += b;
+    b = a;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    return a + b;
+}
+
+// How lane group a's pieces of a K row feed the D / 32 MFMA steps: the k index is a summation index, so any order of the
+// values does that Q is held in, too.  16 bit: step s takes values 32 s + 8 a .. + 7 (a load instruction reads 64 contiguous
+// bytes of each row).  fp8: a 16-byte piece 64 j + 16 a .. + 15 feeds steps 2 j and 2 j + 1.  MXFP4: the a-th quarter of the row.
+template <int KIND, int D>
+__device__ __forceinline__ constexpr int first_value(int step, int a) {
+    return KIND == KEY_16BIT ? 32 * step + 8 * a : KIND == KEY_FP8 ? 64 * (step / 2) + 16 * a + 8 * (step % 2) : (D / 4) * a + 8 * step;
+}
+
+// MANY: more than 16 q heads per kv head - their fragments are read again for every step (from the L1) instead of being held
+template <int QDT, int KIND, int D, bool MANY>
+__global__ __launch_bounds__(256) void attn_weights_kernel(const AttnWeightsParams p) {
+    using P2 = Pack2<QDT>;
+    constexpr int STEPS = D / 32;
+    constexpr int TILES = D <= 128 ? 2 : 1;                // tiles of 16 tokens whose rows are under way together
+    constexpr int LOADS = KIND == KEY_16BIT ? STEPS : KIND == KEY_FP8 ? D / 64 : D > 64 ? D / 128 : 1;     // 16-byte pieces
+    constexpr int MXS = KIND == KEY_MX4 && D == 256 ? 2 : 1;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int a = lane >> 4, c = lane & 15;
+    // rows of less than 128 bytes share cache lines with the neighbouring heads': all heads of a (sequence, share) on one XCD
+    int unit, row;
+    {
+        const int id = (int)blockIdx.x, rows = p.batch * p.shares, T = p.hkv;
+        const int full = rows & ~7;
+        if (id < full * T) {
+            const int blk = id / (8 * T), in = id - blk * 8 * T;
+            unit = in >> 3;
+            row = blk * 8 + (in & 7);
+        } else {
+            const int rest = id - full * T;
+            row = full + rest / T;
+            unit = rest % T;
+        }
+    }
+    const int kvh = unit, b = row / p.shares, share = row - b * p.shares;
+    const int kv_len = min(p.kv_lens[b], p.max_tokens);
+    constexpr int kWgStep = 4 * 16 * TILES;
+    // equal shares of the sequence's own length
+    const int per = max(((kv_len + p.shares - 1) / p.shares + kWgStep - 1) / kWgStep, 1) * kWgStep;
+    const int64_t begin64 = (int64_t)share * per;
+    if (begin64 >= kv_len) return;
+    const int begin = (int)begin64, end = (int)min(begin64 + per, (int64_t)kv_len);
+
+    const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb;
+    const float* lse_row = p.lse + (int64_t)b * p.lse_sb;
+    const int head_tiles = MANY ? (p.group + 15) / 16 : 1;
+    uint4 qf[STEPS];
+    float lse2[4];
+    auto load_q = [&](int ht) {
+        const uint16_t* qp = qrow + (int64_t)(kvh * p.group + min(ht * 16 + c, p.group - 1)) * p.q_sh;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) qf[s] = *reinterpret_cast<const uint4*>(qp + first_value<KIND, D>(s, a));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lse2[i] = lse_row[kvh * p.group + min(ht * 16 + 4 * a + i, p.group - 1)] * kLog2e;
+    };
+    if (!MANY) load_q(0);
+
+    const int32_t* tbl = p.block_table + (int64_t)b * p.tbl_sb;
+    const char* kplane = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh;
+    const uint8_t* splane = p.k_block_scale + (int64_t)kvh * p.bs_sh;
+    float* wrow = p.weights + (int64_t)b * p.w_sb + (int64_t)kvh * p.w_sh;
+    float kscale = 1.f;
+    if (KIND == KEY_FP8 && p.k_scale) kscale = p.k_scale[kvh];
+    const bool softcap = p.soft_cap > 0.f;
+    const float inv_cap = softcap ? 1.0f / p.soft_cap : 0.f;
+
+    auto page_of = [&](int n) { return tbl[p.page_shift < 0 ? n / p.page_size : n >> p.page_shift]; };
+    int32_t pg[TILES];
+    int tok = begin + wave * 16 * TILES;
+    if (tok >= end) return;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) pg[t] = page_of(min(tok + 16 * t + c, end - 1));
+    for (; tok < end; tok += kWgStep) {
+        // rows past the end repeat the last one
+        uint4 raw[TILES][LOADS];
+        uint32_t sc[TILES][MXS];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int n = min(tok + 16 * t + c, end - 1);
+            const int64_t in_page = p.page_shift < 0 ? n % p.page_size : (n & (p.page_size - 1));
+            const char* kp = kplane + (int64_t)pg[t] * p.k_sp + in_page * p.k_st;
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                if constexpr (KIND == KEY_MX4 && D == 64) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(kp + 8 * a);
+                    raw[t][j] = make_uint4(w.x, w.y, 0, 0);
+                } else if constexpr (KIND == KEY_MX4) {
+                    raw[t][j] = *reinterpret_cast<const uint4*>(kp + (D / 8) * a + 16 * j);
+                } else {
+                    raw[t][j] = *reinterpret_cast<const uint4*>(kp + 64 * j + 16 * a);
+                }
+            }
+            if constexpr (KIND == KEY_MX4) {
+                const uint8_t* sp = splane + (int64_t)pg[t] * p.bs_sp + in_page * p.bs_st + (D / 4) * a / kMxBlock;
+#pragma unroll
+                for (int g = 0; g < MXS; ++g) sc[t][g] = sp[g];
+            }
+        }
+        // lane 16 t + c keeps the weight of token c of tile t
+        const int mine = tok + (lane & (16 * TILES - 1));
+        const bool store = lane < 16 * TILES && mine < end;
+        const float old = store ? wrow[mine] : 0.f;
+        const int next = tok + kWgStep;
+        if (next < end) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) pg[t] = page_of(min(next + 16 * t + c, end - 1));
+        }
+        float sum[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) sum[t] = 0.f;
+        for (int ht = 0; ht < head_tiles; ++ht) {
+            if (MANY) load_q(ht);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) {
+                    uint4 kf;
+                    if constexpr (KIND == KEY_16BIT) {
+                        kf = raw[t][st];
+                    } else if constexpr (KIND == KEY_FP8) {
+                        // (k8 * scale) rounded to the q dtype, as the decode does by default
+                        const uint4 w = raw[t][st / 2];
+                        const uint32_t two[2] = {st % 2 ? w.z : w.x, st % 2 ? w.w : w.y};
+                        uint32_t o[4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const f32x2_t k01 = __builtin_amdgcn_cvt_pk_f32_fp8(two[i], false);
+                            const f32x2_t k23 = __builtin_amdgcn_cvt_pk_f32_fp8(two[i], true);
+                            o[2 * i] = P2::pack(k01.x * kscale, k01.y * kscale);
+                            o[2 * i + 1] = P2::pack(k23.x * kscale, k23.y * kscale);
+                        }
+                        kf = make_uint4(o[0], o[1], o[2], o[3]);
+                    } else {
+                        const uint4 w4 = raw[t][st / 4];
+                        const uint32_t w = st % 4 == 0 ? w4.x : st % 4 == 1 ? w4.y : st % 4 == 2 ? w4.z : w4.w;
+                        const float f = mx_scale(sc[t][MXS == 2 ? st / 4 : 0]);
+                        kf = make_uint4(mx_unpack2<QDT, 0>(w, f), mx_unpack2<QDT, 1>(w, f), mx_unpack2<QDT, 2>(w, f), mx_unpack2<QDT, 3>(w, f));
+                    }
+                    s = mma16<QDT>(qf[st], kf, s);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float l2 = softcap ? soft_cap_fn(s[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e : s[i] * p.scale_log2;
+                    const float e = fast_exp2(l2 - lse2[i]);
+                    sum[t] += ht * 16 + 4 * a + i < p.group ? e : 0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) sum[t] = sum_across_rows(sum[t]);
+        if (store) wrow[mine] = old + (TILES == 2 && a == 1 ? sum[TILES - 1] : sum[0]);
+    }
+}
+
+template <int QDT, int KIND, int D>
+int launch_d(const AttnWeightsParams& p, dim3 grid, hipStream_t stream) {
+    if (p.group > 16) hipLaunchKernelGGL((attn_weights_kernel<QDT, KIND, D, true>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((attn_weights_kernel<QDT, KIND, D, false>), grid, dim3(256), 0, stream, p);
+    return (int)hipGetLastError();
+}
+
+template <int QDT, int KIND>
+int launch_kind(const AttnWeightsParams& p, int head_dim, dim3 grid, hipStream_t stream) {
+    switch (head_dim) {
+        case 64: return launch_d<QDT, KIND, 64>(p, grid, stream);
+        case 128: return launch_d<QDT, KIND, 128>(p, grid, stream);
+        case 256: return launch_d<QDT, KIND, 256>(p, grid, stream);
+        default: break;
+    }
+    if constexpr (KIND != KEY_MX4) {
+        if (head_dim == 192) return launch_d<QDT, KIND, 192>(p, grid, stream);
+        if (head_dim == 576) return launch_d<QDT, KIND, 576>(p, grid, stream);
+    }
+    return (int)hipErrorInvalidValue;
+}
+
+}  // namespace
+
+int launch_attn_weights(const AttnWeightsParams& p_in, int head_dim, int q_dtype, int kv_dtype, int num_cus, hipStream_t stream) {
+    AttnWeightsParams p = p_in;
+    // Shares of a sequence per kv head: enough workgroups for eight to a compute unit (they need no merge, so cutting a
+    // sequence finer costs only the loads of q again), at most one per step of 128 tokens.
+    const int64_t units = (int64_t)p.batch * p.hkv;
+    int64_t shares = (8 * (int64_t)num_cus + units - 1) / units;
+    const int64_t most = ((int64_t)p.max_tokens + 127) / 128;
+    if (shares > most) shares = most;
+    if (shares < 1) shares = 1;
+    p.shares = (int32_t)shares;
+    const dim3 grid((unsigned)(units * shares));
+    const bool bf16 = q_dtype == FDK_BF16;
+    if (kv_dtype == FDK_MXFP4)
+        return bf16 ? launch_kind<FDK_BF16, KEY_MX4>(p, head_dim, grid, stream) : launch_kind<FDK_FP16, KEY_MX4>(p, head_dim, grid, stream);
+    if (kv_dtype == FDK_FP8_E4M3)
+        return bf16 ? launch_kind<FDK_BF16, KEY_FP8>(p, head_dim, grid, stream) : launch_kind<FDK_FP16, KEY_FP8>(p, head_dim, grid, stream);
+    return bf16 ? launch_kind<FDK_BF16, KEY_16BIT>(p, head_dim, grid, stream) : launch_kind<FDK_FP16, KEY_16BIT>(p, head_dim, grid, stream);
+}
+
+}  // namespace fdk

@@ -1,0 +1,57 @@
+// Bounding a paged KV cache: attention weights accumulated per cached token, and the eviction of the tokens with the least of
+// it.  Kernel arguments and launchers (fdk_attn_weights.hip, fdk_kv_evict.hip).
+#pragma once
+
+#include "fdk_device.h"
+#include "fdk_mxfp4.h"
+
+namespace fdk {
+
+struct AttnWeightsParams {
+    const void* q;
+    const void* k;
+    const uint8_t* k_block_scale;            // MXFP4 caches
+    const float* k_scale;                    // fp8 caches: [Hkv] or null
+    const int32_t* block_table;
+    const int32_t* kv_lens;
+    const float* lse;
+    float* weights;
+    int64_t q_sb, q_sh;
+    int64_t k_sp, k_st, k_sh;                // bytes
+    int64_t bs_sp, bs_st, bs_sh;             // bytes
+    int64_t tbl_sb, lse_sb;
+    int64_t w_sb, w_sh;
+    int32_t batch, hkv, group;
+    int32_t page_size, page_shift;           // page_shift = log2(page_size) or -1
+    int32_t max_tokens;                      // min(table capacity, weights_len)
+    int32_t shares;                          // workgroups per (sequence, kv head)
+    float scale_log2, sm_scale, soft_cap;
+};
+
+// rows of one tensor of the cache: `cols` pieces of 16 bytes (or single bytes: the block scales)
+struct EvictRows {
+    char* pool;
+    int64_t sp, st, sh;                      // byte strides of the page, token and head axes
+    int32_t cols, bytes;                     // bytes: 16 or 1 per piece
+};
+
+struct EvictParams {
+    EvictRows rows[4];
+    const int32_t* block_table;
+    const int32_t* kv_lens;
+    const float* weights;
+    float* weights_out;
+    int32_t* kept;                           // [B, Hkv, keep]
+    int32_t* plan;                           // [B, Hkv, 4]: first row that moves, first row from outside, new length, unused
+    int32_t* kv_lens_out;
+    int64_t tbl_sb, w_sb, w_sh, wo_sb, wo_sh;
+    int32_t batch, hkv, keep, recent;
+    int32_t weights_len, max_tokens;
+    int32_t page_size, page_shift;
+    int32_t num_tensors;
+};
+
+int launch_attn_weights(const AttnWeightsParams& p, int head_dim, int q_dtype, int kv_dtype, int num_cus, hipStream_t stream);
+int launch_kv_evict(const EvictParams& p, int num_cus, hipStream_t stream);
+
+}  // namespace fdk

@@ -100,6 +100,15 @@ def _stream_handle(stream) -> int:
     return stream.cuda_stream
 
 
+def _launch_on(device: torch.device, stream, fn, args) -> None:
+    """``fn(args, stream)`` of the library with ``device`` current, whatever device is when the caller calls."""
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(C.byref(args), _stream_handle(stream)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(C.byref(args), _stream_handle(stream)))
+
+
 @dataclass
 class SplitKvPlan:
     """Shape-dependent launch constants (the role of the reference's ``algo_info`` dict)."""
@@ -998,7 +1007,7 @@ def _mxfp4_convert(fn, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tenso
         raise ValueError("too many rows")
     a.n, a.x_stride, a.codes_stride, a.scales_stride = (C.c_int32 * 3)(*n), (C.c_int64 * 3)(*xs), (C.c_int64 * 3)(*cs), (C.c_int64 * 3)(*ss)
     a.num_values, a.x_dtype = d, _fdk_dtype(x.dtype, "x")
-    _lib.check(fn(C.byref(a), _stream_handle(stream)))
+    _launch_on(x.device, stream, fn, a)
 
 
 def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,

@@ -11,10 +11,15 @@ Differences, all additions:
   * the pools start zeroed (the reference fills them with random numbers), ``fill="randn"`` restores that;
   * ``dtype=torch.float8_e4m3fn`` keeps 1-byte pools plus per-layer, per-kv-head fp32 scales
     (``k_scale, v_scale [num_layers, Hkv]``, given by the caller);
+  * ``dtype=torch.float4_e2m1fn_x2`` keeps MXFP4 pools: packed codes ``[num_blocks, PAGE_SIZE, Hkv, D/2]`` and, in
+    ``k_block_scale`` / ``v_block_scale``, a scale byte per 32 values, written by ``append``;
   * the lengths are tracked on the host as well (``max_kv_len``), so the decode can be planned for the real
     length without reading ``kv_lens`` back from the GPU (both bounds: the sequences advance together, so
     the decode may use per-sequence chunks) - a hint that is wrong never changes results;
-  * ``append`` / ``decode`` run the two operators of this package on one layer's view.
+  * ``append`` / ``decode`` run the two operators of this package on one layer's view;
+  * ``accumulate`` / ``evict`` keep the cache at a budget: attention weights per cached token, and the eviction of the
+    tokens with the least of them from all layers.  From then on ``append`` takes the tokens' positions from a count of
+    the tokens seen (``next_positions``), not from their places in the cache.
 
 The class itself allocates with torch and launches nothing; it works on any torch device (the operators do not).
 """
@@ -23,6 +28,9 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+
+
+_MXFP4 = getattr(torch, "float4_e2m1fn_x2", None)
 
 
 def alloc_kv_pools(shape, dtype, device, zero: bool = True, v_shape=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -78,6 +86,9 @@ class PagedKVCache:
             raise ValueError("block ids are int32")
         shape = (num_blocks, PAGE_SIZE, num_kv_heads, head_dim)
         fp8 = dtype == torch.float8_e4m3fn
+        self.mxfp4 = dtype == _MXFP4
+        if self.mxfp4 and (fill != "zeros" or head_dim % 32):
+            raise ValueError("an MXFP4 cache starts zeroed and has rows of a multiple of 32 values")
         if fp8:
             if k_scale is None or v_scale is None:
                 raise ValueError("an fp8 cache needs k_scale and v_scale [num_layers, Hkv]")
@@ -89,7 +100,14 @@ class PagedKVCache:
         else:
             self.k_scale = self.v_scale = None
         # (one allocation for both pools, the V pool 256 bytes off the K pool modulo 512: see alloc_kv_pools)
-        self.key_cache, self.value_cache = alloc_kv_pools(shape, dtype, self.device, zero=True)
+        self.k_block_scale = self.v_block_scale = None
+        if self.mxfp4:
+            k, v = alloc_kv_pools(shape[:3] + (head_dim // 2,), torch.uint8, self.device, zero=True)
+            self.key_cache, self.value_cache = k.view(dtype), v.view(dtype)
+            self.k_block_scale = torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.uint8, device=self.device)
+            self.v_block_scale = torch.zeros_like(self.k_block_scale)
+        else:
+            self.key_cache, self.value_cache = alloc_kv_pools(shape, dtype, self.device, zero=True)
         if fill == "randn":
             # drawn on the host so that a seed gives the same cache on every device
             draw = torch.bfloat16 if fp8 else dtype
@@ -99,6 +117,7 @@ class PagedKVCache:
         self.block_tables = perm.reshape(num_layers, batch_size, self.max_num_blocks_per_seq).to(self.device)
         self.kv_lens = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
         self._host_len = 0
+        self._seen = None               # [B] int32: tokens each sequence has seen, once some of them were evicted
 
     # ---- the reference's interface -----------------------------------------------------------------------------
     def inc_offset(self, seq_len: int) -> None:
@@ -107,6 +126,8 @@ class PagedKVCache:
         if seq_len < 0 or self._host_len + seq_len > self.max_length:
             raise ValueError(f"{self._host_len} + {seq_len} tokens exceed max_length = {self.max_length}")
         self.kv_lens += seq_len
+        if self._seen is not None:
+            self._seen += seq_len
         self._host_len += seq_len
 
     def get_layer_kv_cache(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -122,30 +143,72 @@ class PagedKVCache:
 
     @property
     def nbytes(self) -> int:
-        return 2 * self.key_cache.numel() * self.key_cache.element_size()
+        scales = 0 if self.k_block_scale is None else self.k_block_scale.numel()
+        return 2 * (self.key_cache.numel() * self.key_cache.element_size() + scales)
 
     def reset(self) -> None:
         """Forget all tokens; the pages keep their contents and their owners."""
         self.kv_lens.zero_()
         self._host_len = 0
+        self._seen = None
 
     def layer_scales(self, layer_idx: int):
+        if self.mxfp4:
+            return self.k_block_scale, self.v_block_scale          # a byte per row and block: pools like the rows'
         if self.k_scale is None:
             return None, None
         return self.k_scale[layer_idx], self.v_scale[layer_idx]
 
     def append(self, layer_idx: int, qkv: torch.Tensor, q_rms_weight: torch.Tensor, k_rms_weight: torch.Tensor,
                cos_cache: torch.Tensor, sin_cache: torch.Tensor, q_rms_eps: float = 1e-6, k_rms_eps: float = 1e-6,
-               q_norm_rope: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+               q_norm_rope: Optional[torch.Tensor] = None, stream=None, **kwargs) -> torch.Tensor:
         """Norm + rotary + append of ``qkv [B, T, Hq + 2 Hkv, D]`` into one layer, after ``inc_offset(T)``.
-        Returns the normalised, rotated query ``[B, T, Hq, D]``."""
+        ``positions`` / ``rope_sections`` / ``rope_interleaved`` as in ``qk_norm_rope_update_kvcache``; after an eviction
+        ``positions`` defaults to ``next_positions(T)``.  Returns the normalised, rotated query ``[B, T, Hq, D]``."""
         from . import qk_norm_rope_update_kvcache
         if qkv.shape[1] > self._host_len:
             raise ValueError("call inc_offset(T) before append: kv_lens must count the new tokens")
         k, v, table, lens = self.get_layer_kv_cache(layer_idx)
         ks, vs = self.layer_scales(layer_idx)
+        if self._seen is not None and kwargs.get("positions") is None:
+            kwargs["positions"] = self.next_positions(qkv.shape[1])
         return qk_norm_rope_update_kvcache(qkv, k, v, table, lens, q_rms_weight, k_rms_weight, cos_cache, sin_cache,
-                                           q_norm_rope, q_rms_eps, k_rms_eps, k_scale=ks, v_scale=vs, stream=stream)
+                                           q_norm_rope, q_rms_eps, k_rms_eps, k_scale=ks, v_scale=vs, stream=stream, **kwargs)
+
+    def next_positions(self, new_tokens: int) -> torch.Tensor:
+        """Positions ``[B, T]`` int32 of the T tokens that ``inc_offset(T)`` has just counted: how many tokens their
+        sequence had seen before them, evicted ones among them."""
+        seen = self.kv_lens if self._seen is None else self._seen
+        return seen[:, None] - new_tokens + torch.arange(new_tokens, dtype=torch.int32, device=self.device)
+
+    def accumulate(self, layer_idx: int, q: torch.Tensor, lse: torch.Tensor, sm_scale: float, weights: torch.Tensor, **kwargs):
+        """``accumulate_attention_weights`` of a decode's query and lse over one layer; weights ``[B, Hkv, S]``."""
+        from . import accumulate_attention_weights
+        k, _, table, lens = self.get_layer_kv_cache(layer_idx)
+        ks, _ = self.layer_scales(layer_idx)
+        if ks is not None:
+            kwargs.setdefault("k_scale", ks)
+        return accumulate_attention_weights(q, k, table, lens, lse, sm_scale, weights, **kwargs)
+
+    def evict(self, weights: torch.Tensor, keep: int, recent: int, stream=None) -> Optional[torch.Tensor]:
+        """Bring every layer back to at most ``keep`` tokens by its weights ``[num_layers, B, Hkv, S]``, which move along
+        (see ``evict_kvcache``).  Returns ``kept [num_layers, B, Hkv, keep]``, or None if nothing had to go."""
+        from . import evict_kvcache
+        if weights.dim() != 4 or weights.shape[0] != self.num_layers or weights.shape[3] < self._host_len:
+            raise ValueError(f"weights must be [{self.num_layers}, B, Hkv, S] with S >= {self._host_len} tokens")
+        if self._host_len <= keep:
+            return None
+        kept = torch.empty((self.num_layers, self.batch_size, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
+        scales = {} if not self.mxfp4 else dict(k_scale=self.k_block_scale, v_scale=self.v_block_scale)
+        seen = self.kv_lens.clone() if self._seen is None else self._seen
+        for layer in range(self.num_layers):
+            # (the layers share kv_lens: the last one changes it)
+            lens_out = self.kv_lens if layer == self.num_layers - 1 else None
+            evict_kvcache(self.key_cache, self.value_cache, self.block_tables[layer], self.kv_lens, weights[layer], keep, recent,
+                          weights_out=weights[layer], kept=kept[layer], kv_lens_out=lens_out, stream=stream, **scales)
+        self._seen = seen
+        self._host_len = keep
+        return kept
 
     def decode(self, layer_idx: int, q: torch.Tensor, sm_scale: float, **kwargs):
         """``flash_decode`` of ``q [B, Hq, D]`` over one layer, planned for the host-known length.
