@@ -286,6 +286,11 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
     return FDK_OK;
 }
 
+int mx_kv_heads_per_wg(const fdk_decode_args* a) {
+    const bool neighbours = a->k_stride_head == a->head_dim / 2 && a->v_stride_head == a->head_dim / 2;
+    return neighbours && a->head_dim <= 128 && a->num_kv_heads % 2 == 0 ? 2 : 1;
+}
+
 int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
     const int group = a->num_q_heads / a->num_kv_heads;
     int algo = a->algo;
@@ -313,7 +318,9 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
     int units_per_seq;
     const int tile_heads = algo == FDK_ALGO_MFMA ? fdk::mfma_heads_per_wg(group, a->head_dim + v_dim(a), a->kv_dtype) : 16;   // q heads of a kv head per workgroup
     if (algo == FDK_ALGO_MFMA) {
-        kv_heads_per_wg = fdk::mfma_kv_heads_per_wg(batch, a->num_kv_heads, group, num_cus, a->head_dim + v_dim(a), a->kv_dtype);
+        kv_heads_per_wg = a->kv_dtype == FDK_MXFP4
+                              ? mx_kv_heads_per_wg(a)
+                              : fdk::mfma_kv_heads_per_wg(batch, a->num_kv_heads, group, num_cus, a->head_dim + v_dim(a), a->kv_dtype);
         units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
     } else {
         units_per_seq = fdk::valu_units_per_seq(a->num_kv_heads, group, heads_contiguous, a->kv_dtype);
@@ -353,7 +360,8 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
         }
         if (rebalance) {
             kv_heads_per_wg = a->num_kv_heads % 2 ? 1 : 2;
-            if (tile_heads > 16 || a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = 1;
+            if (tile_heads > 16) kv_heads_per_wg = 1;
+            if (a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = mx_kv_heads_per_wg(a);
             units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
         }
     }

@@ -17,6 +17,7 @@
     // workgroups with an odd number of kv heads are mapped so that those neighbours run on one XCD (one L2 fetches the
     // line once; spread over the XCDs in dispatch order every head's L2 fetched both of its partial lines).
     constexpr bool kRowsShareLines = !kOneSegment && FP8 && (DK % 128 != 0 || DV % 128 != 0);
+    constexpr bool kScalesShareLines = false;
     static_assert(kOneSegment || (NBUF == 1 && !PROBE && (PM == PM_TILE || PM == PM_ROW)), "not built");
     static_assert(DK >= DV && DK % 32 == 0 && DV % 16 == 0, "K rows at least as long as V rows");
     constexpr int NJ = R::NJ;                  // (one segment)

@@ -56,6 +56,7 @@ __global__ __launch_bounds__(64 * kSharedWaves) void splitkv_mfma_shared_kernel(
     static_assert(DK % 64 == 0 && DV % 64 == 0, "the LDS swizzle acts on groups of eight 16-byte chunks");
     constexpr bool kOneSegment = false;        // (fdk_splitkv_mfma_work.h: several head tiles of a kv head go to one XCD)
     constexpr bool kRowsShareLines = false;    // (16-bit rows: whole 128-byte lines per kv head)
+    constexpr bool kScalesShareLines = false;
     constexpr int kTileHeads = kSharedTileHeads;
     constexpr bool kFirstPieceStraight = true;  // (fdk_splitkv_mfma_work.h)
     constexpr int NW = kSharedWaves;

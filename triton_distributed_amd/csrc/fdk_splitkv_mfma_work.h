@@ -2,7 +2,8 @@
 // each kernel's body (the kernel definitions include this file after they have defined run_piece, write_empty_rows
 // and: p, lane, wave, nh = kv heads per workgroup, hl = this wavefront's kv head within the block, tix = its index among
 // the wavefronts of that head, s_next = an int in LDS, kTileHeads = q heads per head tile, kOneSegment, MODE,
-// kFirstPieceStraight = whether a share's first piece gets straight-line code of its own, see below).
+// kRowsShareLines / kScalesShareLines = whether the rows of neighbouring kv heads / the block scales of all kv heads are parts
+// of the same lines, kFirstPieceStraight = whether a share's first piece gets straight-line code of its own, see below).
     // ---- work distribution --------------------------------------------------------------------------------------
     // Chunk mode: item -> (sequence, split, kv-head block, q-head tile), partial row (b, head, split); one item per
     // workgroup, or (persistent) a fixed set of workgroups that pull items from a queue: counters[0] is its head,
@@ -38,7 +39,7 @@
                     ht = blockIdx.x % p.head_tiles;
                     hgb = blockIdx.x / p.head_tiles;
                 }
-            } else if (kRowsShareLines && (nh & 1) && p.hg_blocks > 1) {
+            } else if (kRowsShareLines && ((nh & 1) || kScalesShareLines) && p.hg_blocks > 1) {
                 // every unit of a (sequence, split) on one XCD: neighbouring kv heads share 128-byte lines
                 int row, unit;
                 tiles_on_one_xcd((int)(blockIdx.x + p.grid_x * (blockIdx.y + p.num_splits * blockIdx.z)),
@@ -140,7 +141,7 @@
         int b = 0, before = 0, gb = 1;                // sequence of x, granules of the sequences before it, its granules
         int wc_of_wg = blockIdx.y, bu_of_wg = blockIdx.x;   // grid = (units, shares)
         if constexpr (!kOneSegment) {
-            if (kRowsShareLines && (nh & 1) && p.hg_blocks > 1) {   // every unit of a share on one XCD
+            if (kRowsShareLines && ((nh & 1) || kScalesShareLines) && p.hg_blocks > 1) {   // every unit of a share on one XCD
                 tiles_on_one_xcd((int)(blockIdx.x + p.grid_x * blockIdx.y), p.shares, p.grid_x, wc_of_wg, bu_of_wg);
             } else if (p.head_tiles > 1) {                  // the q-head tiles of a (share, kv-head block) on one XCD
                 int row, tile;

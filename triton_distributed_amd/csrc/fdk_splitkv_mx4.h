@@ -27,6 +27,7 @@ namespace fdk {
 
 namespace {
 
+constexpr int kWaves = 8;                  // wavefronts of a workgroup
 constexpr int kStep = 32;                  // tokens per wavefront and step: two tiles of 16 rows, one k-step of P V
 
 template <int D>
@@ -37,10 +38,13 @@ struct Mx4Tile {                           // one step in registers, as loaded
     uint32_t k[2][KW];
     uint32_t ks[2][KS];
     uint32_t v[8][VW];
-    uint32_t vs[8];
+    static constexpr int VS = D == 256 ? 2 : 1;           // V scales a lane loads per tile (of the four tokens of a lane group)
+    uint32_t vs[2][VS];
 };
 
-template <int QDT, int PM, int D, int MODE>
+// NH: kv heads of a workgroup (neighbours in memory: their rows share lines).  STREAM: every line is one workgroup's alone, and
+// is loaded with the non-temporal hint; otherwise plain loads leave the lines in the L2 for the next reader.
+template <int QDT, int PM, int D, int MODE, int NH, bool STREAM>
 __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, const Mx4Scales x) {
     static_assert(PM == PM_TILE || PM == PM_ROW, "page numbers per tile of 16 tokens, or per row");
     using P2 = Pack2<QDT>;
@@ -50,21 +54,21 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     constexpr int KSTEPS = D / 32;             // MFMA steps of a K row
     constexpr int kTileHeads = 16;
     constexpr bool kOneSegment = false;        // (fdk_splitkv_mfma_work.h: no single-launch form, units mapped to XCDs)
-    constexpr bool kRowsShareLines = true;
+    constexpr bool kRowsShareLines = true, kScalesShareLines = true;
     constexpr bool kFirstPieceStraight = true;
-    extern __shared__ __attribute__((aligned(16))) char lds[];      // [nw][D * 64] then m[nw][16], l[nw][16], s_next
+    extern __shared__ __attribute__((aligned(16))) char lds[];      // [nw][NH][D * 64] then m[nw][NH][16], l[nw][NH][16], s_next
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int a = lane >> 4;
     const int c = lane & 15;
     const int nw = p.wavefronts;
-    const int nh = 1, hl = 0;                  // one kv head per workgroup
+    const int nh = NH, hl = 0;                 // kv heads of a workgroup: every wavefront works on all of them
     const int tix = wave;
-    constexpr int kScratch = D * 64;           // a wavefront's 16 output rows in fp32
-    float* sm_m = reinterpret_cast<float*>(lds + nw * kScratch);
-    float* sm_l = sm_m + nw * 16;
-    int* const s_next = reinterpret_cast<int*>(sm_l + nw * 16);
+    constexpr int kScratch = D * 64;           // 16 output rows in fp32: a wavefront's for one kv head
+    float* sm_m = reinterpret_cast<float*>(lds + nw * NH * kScratch);
+    float* sm_l = sm_m + nw * NH * 16;
+    int* const s_next = reinterpret_cast<int*>(sm_l + nw * NH * 16);
 
     // out = 0, lse = -inf for the q heads [head0, head0 + heads_here) of an empty sequence; one wavefront
     auto write_empty_rows = [&](const int b, const int head0, const int heads_here) {
@@ -79,19 +83,23 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
         }
     };
 
-    // One piece: tokens [c_start, min(c_limit, kv_len)) of sequence b for kv head kvh and q-head tile ht; c_start is a
-    // multiple of 16.  Partial results of head g of the tile go to row prow0 + g * prow_step of the workspace.
-    auto run_piece = [&](const int b, const int kvh, const int ht, const int c_start, const int c_limit, const int64_t prow0,
+    // One piece: tokens [c_start, min(c_limit, kv_len)) of sequence b for kv heads NH hgb .. NH hgb + NH - 1 and q-head tile ht;
+    // c_start is a multiple of 16.  Partial results of head g of the tile go to row prow0 + g * prow_step of the workspace,
+    // those of the next kv head to the rows kv_step further on.
+    const int64_t kv_step = MODE == WM_SHARES ? p.heads_per_tile : (int64_t)p.group * p.num_splits;
+    auto run_piece = [&](const int b, const int hgb, const int ht, const int c_start, const int c_limit, const int64_t prow0,
                          const int prow_step, MergeRows) {
-    const int head0 = kvh * p.group + ht * kTileHeads;
+    const int kvh = hgb * NH;
+    const int head0 = kvh * p.group + ht * kTileHeads;                     // + h * group for kv head kvh + h
     const int heads_here = min(kTileHeads, p.group - ht * kTileHeads);
     // Q^T: lane (h = c, a) holds q[h][(D/4) a + 8 ks .. + 7] (columns past the group repeat its last head, and are not stored)
-    uint4 qb[KSTEPS];
-    {
-        const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb +
-                             (int64_t)(head0 + min(c, heads_here - 1)) * p.q_sh + (D / 4) * a;
+    uint4 qb[NH][KSTEPS];
 #pragma unroll
-        for (int ks = 0; ks < KSTEPS; ++ks) qb[ks] = *reinterpret_cast<const uint4*>(qp + 8 * ks);
+    for (int h = 0; h < NH; ++h) {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb +
+                             (int64_t)(head0 + h * p.group + min(c, heads_here - 1)) * p.q_sh + (D / 4) * a;
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks) qb[h][ks] = *reinterpret_cast<const uint4*>(qp + 8 * ks);
     }
     const ConstI32 tbl = as_const(p.block_table + (int64_t)b * p.tbl_sb);
     const int pmask = p.page_size - 1;
@@ -113,7 +121,10 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     fetch_pages(tix + nw, p.max_tokens - 1, pb);
     const int kv_len = min(as_const(p.kv_lens)[b], p.max_tokens);
     if (c_start >= kv_len) {
-        if (p.direct && tix == 0) write_empty_rows(b, head0, heads_here);
+        if (p.direct && tix == 0) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h) write_empty_rows(b, head0 + h * p.group, heads_here);
+        }
         return;
     }
     const int c_end = min(c_limit, kv_len);
@@ -127,107 +138,146 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     const int krow = (c >> 2) + 4 * (c & 3);                  // the token (of 16) that row c of S^T belongs to
     const uint32_t kbyte = (uint32_t)(a * (D / 8)), vbyte = (uint32_t)(c * (D / 32));
     const uint32_t ksbyte = (uint32_t)((D / 4) * a / kMxBlock), vsbyte = (uint32_t)(DB * c / kMxBlock);
+    // V scales: four neighbouring lanes hold values of one block (D = 256: two lanes) and need the scales of the same four
+    // tokens of each tile; each lane loads one token's (two tokens') and they exchange (v_scales).
+    const int vstok = a + 4 * (T::VS == 1 ? c & 3 : c & 1);               // + 8 g: the token of scale g
 
+    auto load = [&](auto type_tag, const char* at) {
+        using V = decltype(type_tag);
+        if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(at));
+        else return *reinterpret_cast<const V*>(at);
+    };
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
     auto load_k = [&](const char* at, uint32_t (&dst)[T::KW]) {
         if constexpr (D == 64) {
-            const uint2 w = *reinterpret_cast<const uint2*>(at);
+            const u32x2_t w = load(u32x2_t(), at);
             dst[0] = w.x; dst[1] = w.y;
         } else {
 #pragma unroll
             for (int j = 0; j < T::KW; j += 4) {
-                const uint4 w = *reinterpret_cast<const uint4*>(at + 4 * j);
+                const u32x4_t w = load(u32x4_t(), at + 4 * j);
                 dst[j] = w.x; dst[j + 1] = w.y; dst[j + 2] = w.z; dst[j + 3] = w.w;
             }
         }
     };
     auto load_v = [&](const char* at, uint32_t (&dst)[T::VW]) {
         if constexpr (D == 64) {
-            dst[0] = *reinterpret_cast<const uint16_t*>(at);
+            dst[0] = load(uint16_t(), at);
         } else if constexpr (D == 128) {
-            dst[0] = *reinterpret_cast<const uint32_t*>(at);
+            dst[0] = load(uint32_t(), at);
         } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(at);
+            const u32x2_t w = load(u32x2_t(), at);
             dst[0] = w.x; dst[1] = w.y;
         }
     };
+    auto load_byte = [&](const char* at) { return (uint32_t) * reinterpret_cast<const uint8_t*>(at); };
     // per-lane byte offsets of a tile's rows from its first row (PM_TILE)
-    uint32_t voff[4], vsoff[4];
+    uint32_t voff[4];
+    const uint32_t vsoff = (uint32_t)(vstok * x.v_st) + vsbyte;
     const uint32_t koff = (uint32_t)(krow * p.k_st) + kbyte;
     const uint32_t ksoff = (uint32_t)(krow * x.k_st) + ksbyte;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        voff[i] = (uint32_t)((a + 4 * i) * p.v_st) + vbyte;
-        vsoff[i] = (uint32_t)((a + 4 * i) * x.v_st) + vsbyte;
-    }
-    // rows of step t; CLAMP: positions past c_end repeat the last token (the partial last step)
-    auto issue = [&](int t, const Pages& pi, T& r, auto clamp_tag) {
-        constexpr bool CLAMP = decltype(clamp_tag)::value;
-        const int tok0 = c_start + t * kStep;
-        if constexpr (PM == PM_TILE && !CLAMP) {
+    for (int i = 0; i < 4; ++i) voff[i] = (uint32_t)((a + 4 * i) * p.v_st) + vbyte;
+    // byte offset of a row: page strides and in-page offsets are below 4 GiB, one 32 x 32 -> 64 bit multiply-add
+    auto offset = [&](int64_t sp, int64_t st, uint32_t pg, uint32_t slot) {
+        return (uint64_t)pg * (uint32_t)sp + (uint64_t)(slot * (uint32_t)st);
+    };
+    // page and slot of row 0 .. 31 of step t; CLAMP: positions past c_end repeat the last token (the partial last step)
+    auto place = [&](int t, const Pages& pi, int row, auto clamp_tag, uint32_t& pg, uint32_t& slot) {
+        int n = c_start + t * kStep + row;
+        if (decltype(clamp_tag)::value) n = min(n, c_end - 1);
+        slot = (uint32_t)(p.page_shift < 0 ? n % p.page_size : (n & pmask));
+        if constexpr (PM == PM_TILE) pg = (uint32_t)(row < 16 ? pi.pg[0] : pi.pg[PM == PM_TILE ? 1 : 0]);
+        else pg = (uint32_t)__shfl(pi.pg[0], row, 64);
+    };
+    // The rows of step t.  The kv heads of a workgroup are neighbours: their rows are parts of the same lines, requested one
+    // right after the other.
+    auto issue_k = [&](int t, const Pages& pi, T (&r)[NH], auto clamp_tag) {
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int64_t pg = pi.pg[hf];
-                const int64_t slot = (tok0 + 16 * hf) & pmask;
-                const char* kp = kplane + pg * p.k_sp + slot * p.k_st;
-                const char* ksp = ksplane + pg * x.k_sp + slot * x.k_st;
-                load_k(kp + koff, r.k[hf]);
-#pragma unroll
-                for (int g = 0; g < T::KS; ++g) r.ks[hf][g] = *reinterpret_cast<const uint8_t*>(ksp + ksoff + g);
+        for (int hf = 0; hf < 2; ++hf) {
+            uint32_t pg, slot;
+            if constexpr (PM == PM_TILE && !decltype(clamp_tag)::value) {
+                pg = (uint32_t)pi.pg[hf];                                     // (wave-uniform: the lanes' part is an offset)
+                slot = (uint32_t)((c_start + t * kStep + 16 * hf) & pmask);
+            } else {
+                place(t, pi, 16 * hf + krow, clamp_tag, pg, slot);
             }
+            constexpr bool UNIFORM = PM == PM_TILE && !decltype(clamp_tag)::value;
+            const char* kp = kplane + offset(p.k_sp, p.k_st, pg, slot);
+            const char* ksp = ksplane + offset(x.k_sp, x.k_st, pg, slot);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int64_t pg = pi.pg[hf];
-                const int64_t slot = (tok0 + 16 * hf) & pmask;
-                const char* vp = vplane + pg * p.v_sp + slot * p.v_st;
-                const char* vsp = vsplane + pg * x.v_sp + slot * x.v_st;
+            for (int h = 0; h < NH; ++h) load_k(kp + h * p.k_sh + (UNIFORM ? koff : kbyte), r[h].k[hf]);
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+                for (int g = 0; g < T::KS; ++g) r[h].ks[hf][g] = load_byte(ksp + h * x.k_sh + (UNIFORM ? ksoff : ksbyte) + g);
+        }
+    };
+    auto issue_v = [&](int t, const Pages& pi, T (&r)[NH], auto clamp_tag) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            if constexpr (PM == PM_TILE && !decltype(clamp_tag)::value) {
+                const uint32_t pg = (uint32_t)pi.pg[hf], slot = (uint32_t)((c_start + t * kStep + 16 * hf) & pmask);
+                const char* vp = vplane + offset(p.v_sp, p.v_st, pg, slot);
+                const char* vsp = vsplane + offset(x.v_sp, x.v_st, pg, slot);
+#pragma unroll
+                for (int g = 0; g < T::VS; ++g)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) r[h].vs[hf][g] = load_byte(vsp + h * x.v_sh + (uint32_t)(8 * g * x.v_st) + vsoff);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) load_v(vp + h * p.v_sh + voff[i], r[h].v[4 * hf + i]);
+            } else {
+#pragma unroll
+                for (int g = 0; g < T::VS; ++g) {
+                    uint32_t pg, slot;
+                    place(t, pi, 16 * hf + vstok + 8 * g, clamp_tag, pg, slot);
+                    const char* vsp = vsplane + offset(x.v_sp, x.v_st, pg, slot) + vsbyte;
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) r[h].vs[hf][g] = load_byte(vsp + h * x.v_sh);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    load_v(vp + voff[i], r.v[4 * hf + i]);
-                    r.vs[4 * hf + i] = *reinterpret_cast<const uint8_t*>(vsp + vsoff[i]);
+                    uint32_t pg, slot;
+                    place(t, pi, 16 * hf + a + 4 * i, clamp_tag, pg, slot);
+                    const char* vp = vplane + offset(p.v_sp, p.v_st, pg, slot) + vbyte;
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) load_v(vp + h * p.v_sh, r[h].v[4 * hf + i]);
                 }
-            }
-        } else {
-            // a row's page and slot; row = 0 .. 31 of the step
-            auto place = [&](int row, uint32_t& pg, uint32_t& slot) {
-                int n = tok0 + row;
-                if (CLAMP) n = min(n, c_end - 1);
-                slot = (uint32_t)(p.page_shift < 0 ? n % p.page_size : (n & pmask));
-                if constexpr (PM == PM_TILE) pg = (uint32_t)(row < 16 ? pi.pg[0] : pi.pg[PM == PM_TILE ? 1 : 0]);
-                else pg = (uint32_t)__shfl(pi.pg[0], row, 64);
-            };
-            // (page strides and in-page offsets are below 4 GiB: one 32 x 32 -> 64 bit multiply-add per address)
-            auto at = [&](const char* plane, int64_t sp, int64_t st, uint32_t pg, uint32_t slot) {
-                return plane + ((uint64_t)pg * (uint32_t)sp + (uint64_t)(slot * (uint32_t)st));
-            };
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                uint32_t pg, slot;
-                place(16 * hf + krow, pg, slot);
-                load_k(at(kplane, p.k_sp, p.k_st, pg, slot) + kbyte, r.k[hf]);
-#pragma unroll
-                for (int g = 0; g < T::KS; ++g)
-                    r.ks[hf][g] = *reinterpret_cast<const uint8_t*>(at(ksplane, x.k_sp, x.k_st, pg, slot) + ksbyte + g);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t pg, slot;
-                place(16 * (j >> 2) + a + 4 * (j & 3), pg, slot);
-                load_v(at(vplane, p.v_sp, p.v_st, pg, slot) + vbyte, r.v[j]);
-                r.vs[j] = *reinterpret_cast<const uint8_t*>(at(vsplane, x.v_sp, x.v_st, pg, slot) + vsbyte);
             }
         }
     };
 
-    float m_run = -INFINITY, l_run = 0.f;       // for head c; l_run is this lane group's share of the sum
-    f32x4_t acc[DB];                             // acc[db][i] = O[h = c][DB (4 a + i) + db]
+    float m_run[NH], l_run[NH];                  // for head c; l_run is this lane group's share of the sum
+    f32x4_t acc[NH][DB];                         // acc[h][db][i] = O[head c of kv head h][DB (4 a + i) + db]
 #pragma unroll
-    for (int db = 0; db < DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < NH; ++h) {
+        m_run[h] = -INFINITY;
+        l_run[h] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[h][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
 
+    // the scales of the lane group's four tokens, from the four lanes (two pairs of lanes) that loaded them
+    auto v_scales = [&](const uint32_t (&in)[T::VS], float* sc) {
+        if constexpr (T::VS == 1) {
+            const float x0 = mx_scale(in[0]);
+            sc[0] = dpp_mov<0x00>(x0);                         // quad_perm [0,0,0,0] ...
+            sc[1] = dpp_mov<0x55>(x0);
+            sc[2] = dpp_mov<0xAA>(x0);
+            sc[3] = dpp_mov<0xFF>(x0);
+        } else {
+            const float x0 = mx_scale(in[0]), x1 = mx_scale(in[1]);
+            sc[0] = dpp_mov<0xA0>(x0);                         // quad_perm [0,0,2,2]
+            sc[1] = dpp_mov<0xF5>(x0);                         // quad_perm [1,1,3,3]
+            sc[2] = dpp_mov<0xA0>(x1);
+            sc[3] = dpp_mov<0xF5>(x1);
+        }
+    };
     auto mma = [&](uint4 av, uint4 bv, f32x4_t cv) { return Mma<QDT>::qk(av, bv, cv); };     // 16 x 16 x 32
-    auto compute = [&](int t, const T& r, auto masked_tag) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
-        // ---- S^T[token][head] = K Q^T, two tiles of 16 tokens ----
-        float sv[8];
+    // ---- S^T[token][head] = K Q^T, two tiles of 16 tokens: sv[4 hf + i] is token 16 hf + a + 4 i ----
+    auto scores = [&](const T& r, const uint4 (&q)[KSTEPS], float (&sv)[8]) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             f32x4_t s = {0.f, 0.f, 0.f, 0.f};
@@ -236,12 +286,14 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
                 const float sc = mx_scale(r.ks[hf][T::KS == 2 ? ks / 4 : 0]);
                 const uint32_t w = r.k[hf][ks];
                 s = mma(make_uint4(mx_unpack2<QDT, 0>(w, sc), mx_unpack2<QDT, 1>(w, sc), mx_unpack2<QDT, 2>(w, sc),
-                                   mx_unpack2<QDT, 3>(w, sc)), qb[ks], s);
+                                   mx_unpack2<QDT, 3>(w, sc)), q[ks], s);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) sv[4 * hf + i] = s[i];
         }
-        // ---- online softmax for head c over this lane group's eight tokens ----
+    };
+    // ---- online softmax for head c over this lane group's eight tokens; the probabilities as operand B of P V ----
+    auto softmax = [&](int t, float (&sv)[8], int h, auto masked_tag) {
         if (softcap) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sv[i] = soft_cap_fn(sv[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e;
@@ -249,7 +301,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
 #pragma unroll
             for (int i = 0; i < 8; ++i) sv[i] *= p.scale_log2;
         }
-        if (MASKED) {
+        if (decltype(masked_tag)::value) {
             const int tok0 = c_start + t * kStep;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -259,24 +311,26 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
         mx = max_across_rows(mx);
         // The running maximum moves only when a step exceeds it by more than 2^8: probabilities of up to 256 are as exact
         // in 16 bits and in the fp32 sums as those below 1, and the accumulators are rescaled a few times per piece.
-        if (__builtin_amdgcn_ballot_w64(mx > m_run + 8.0f) != 0) {
-            const float m_new = fmaxf(m_run, mx);
-            const float alpha = fast_exp2(m_run - m_new);
-            l_run *= alpha;
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[h] + 8.0f) != 0) {
+            const float m_new = fmaxf(m_run[h], mx);
+            const float alpha = fast_exp2(m_run[h] - m_new);
+            l_run[h] *= alpha;
 #pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
-            m_run = m_new;
+            for (int db = 0; db < DB; ++db) acc[h][db] *= alpha;
+            m_run[h] = m_new;
         }
         float pr[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(sv[i] - m_run);
-        l_run += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(sv[i] - m_run[h]);
+        l_run[h] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
         // probabilities rounded to the q dtype, as the 16-bit kernels do; the sum above is of the unrounded ones
-        const uint4 pv = make_uint4(P2::pack(pr[0], pr[1]), P2::pack(pr[2], pr[3]), P2::pack(pr[4], pr[5]), P2::pack(pr[6], pr[7]));
-        // ---- O^T[value][head] += V^T P^T ----
+        return make_uint4(P2::pack(pr[0], pr[1]), P2::pack(pr[2], pr[3]), P2::pack(pr[4], pr[5]), P2::pack(pr[6], pr[7]));
+    };
+    // ---- O^T[value][head] += V^T P^T ----
+    auto values = [&](const T& r, const uint4 pv, f32x4_t (&o)[DB]) {
         float sc[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = mx_scale(r.vs[j]);
+        for (int hf = 0; hf < 2; ++hf) v_scales(r.vs[hf], sc + 4 * hf);
         auto pair = [&](auto byte_tag, int w, int db) {        // column blocks db, db + 1: byte `byte_tag` of the V words
             constexpr int BY = decltype(byte_tag)::value;
             uint32_t u[8];
@@ -288,8 +342,8 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
                 lo[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x05040100u);
                 hi[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
             }
-            acc[db] = mma(make_uint4(lo[0], lo[1], lo[2], lo[3]), pv, acc[db]);
-            acc[db + 1] = mma(make_uint4(hi[0], hi[1], hi[2], hi[3]), pv, acc[db + 1]);
+            o[db] = mma(make_uint4(lo[0], lo[1], lo[2], lo[3]), pv, o[db]);
+            o[db + 1] = mma(make_uint4(hi[0], hi[1], hi[2], hi[3]), pv, o[db + 1]);
         };
 #pragma unroll
         for (int w = 0; w < T::VW; ++w) {
@@ -302,67 +356,114 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
         }
     };
 
-    // ---- pipeline: two register buffers, the next step's rows are requested before a step is worked on; page numbers run
-    // a step further ahead ----
+    // ---- pipeline ----
+    // One kv head: two register buffers, a step's rows are requested a whole step ahead.  Two kv heads (twice the registers):
+    // one buffer, the K registers take the next step's rows as soon as the logits are there, the V registers after P V.  Page
+    // numbers run a step further ahead: vector loads of them in front of the rows, scalar ones behind (see
+    // fdk_splitkv_mfma_body.h).
     const int n_full = (c_end - c_start) / kStep;
     {
-        T ra, rb;
+        T r[NH];
         int t = tix;
         const int st = nw;
-        if (t < n_full) issue(t, pa, ra, BoolTag<false>());
-        while (t + 2 * st < n_full) {
-            fetch_pages(t + 2 * st, p.max_tokens - 1, pa);
-            issue(t + st, pb, rb, BoolTag<false>());
-            compute(t, ra, BoolTag<false>());
-            fetch_pages(t + 3 * st, p.max_tokens - 1, pb);
-            issue(t + 2 * st, pa, ra, BoolTag<false>());
-            compute(t + st, rb, BoolTag<false>());
-            t += 2 * st;
+        if (t < n_full) {
+            issue_k(t, pa, r, BoolTag<false>());
+            issue_v(t, pa, r, BoolTag<false>());
         }
-        if (t + st < n_full) {
-            issue(t + st, pb, rb, BoolTag<false>());
-            compute(t, ra, BoolTag<false>());
-            compute(t + st, rb, BoolTag<false>());
-        } else if (t < n_full) {
-            compute(t, ra, BoolTag<false>());
+        if constexpr (NH == 1) {
+            T r2[NH];
+            auto work = [&](int tw, const T (&rw)[NH]) {
+                float sv[8];
+                scores(rw[0], qb[0], sv);
+                values(rw[0], softmax(tw, sv, 0, BoolTag<false>()), acc[0]);
+            };
+            while (t + 2 * st < n_full) {
+                fetch_pages(t + 2 * st, p.max_tokens - 1, pa);
+                issue_k(t + st, pb, r2, BoolTag<false>());
+                issue_v(t + st, pb, r2, BoolTag<false>());
+                work(t, r);
+                fetch_pages(t + 3 * st, p.max_tokens - 1, pb);
+                issue_k(t + 2 * st, pa, r, BoolTag<false>());
+                issue_v(t + 2 * st, pa, r, BoolTag<false>());
+                work(t + st, r2);
+                t += 2 * st;
+            }
+            if (t + st < n_full) {
+                issue_k(t + st, pb, r2, BoolTag<false>());
+                issue_v(t + st, pb, r2, BoolTag<false>());
+                work(t, r);
+                work(t + st, r2);
+            } else if (t < n_full) {
+                work(t, r);
+            }
+        } else {
+            constexpr bool kIdsFirst = PM == PM_ROW;
+            while (t < n_full) {
+                const int tn = t + st;
+                const bool more = tn < n_full;
+                if (kIdsFirst) fetch_pages(tn + st, p.max_tokens - 1, pa);
+                float sv[NH][8];
+#pragma unroll
+                for (int h = 0; h < NH; ++h) scores(r[h], qb[h], sv[h]);
+                if (more) issue_k(tn, pb, r, BoolTag<false>());
+                uint4 pv[NH];
+#pragma unroll
+                for (int h = 0; h < NH; ++h) pv[h] = softmax(t, sv[h], h, BoolTag<false>());
+#pragma unroll
+                for (int h = 0; h < NH; ++h) values(r[h], pv[h], acc[h]);
+                if (more) issue_v(tn, pb, r, BoolTag<false>());
+                if (!kIdsFirst) fetch_pages(tn + st, p.max_tokens - 1, pa);
+                pb = pa;
+                t = tn;
+            }
         }
         if (n_full * kStep < c_end - c_start && n_full % nw == tix) {
             fetch_pages(n_full, c_end - 1, pa);
-            issue(n_full, pa, ra, BoolTag<true>());
-            compute(n_full, ra, BoolTag<true>());
+            issue_k(n_full, pa, r, BoolTag<true>());
+            issue_v(n_full, pa, r, BoolTag<true>());
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                float sv[8];
+                scores(r[h], qb[h], sv);
+                values(r[h], softmax(n_full, sv, h, BoolTag<true>()), acc[h]);
+            }
         }
     }
 
     // ---- merge: lane groups (sum of l), then the wavefronts through LDS ----
     // Block e = i (DB / 4) + q of a wavefront's scratch holds, per lane, its values DB (4 a + i) + 4 q .. + 3 of head c: every
     // LDS instruction touches one contiguous kilobyte, and a merging lane stores four consecutive values.
-    l_run += __shfl_xor(l_run, 16, 64);
-    l_run += __shfl_xor(l_run, 32, 64);
     const bool live = c < heads_here;
-    float4* my_o = reinterpret_cast<float4*>(lds + wave * kScratch);
-    if (live) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int h = 0; h < NH; ++h) {
+        l_run[h] += __shfl_xor(l_run[h], 16, 64);
+        l_run[h] += __shfl_xor(l_run[h], 32, 64);
+        float4* my_o = reinterpret_cast<float4*>(lds + (wave * NH + h) * kScratch);
+        if (live) {
 #pragma unroll
-            for (int q = 0; q < DB / 4; ++q)
-                my_o[(i * (DB / 4) + q) * 64 + lane] = make_float4(acc[4 * q][i], acc[4 * q + 1][i], acc[4 * q + 2][i], acc[4 * q + 3][i]);
-        if (a == 0) {
-            sm_m[wave * 16 + c] = m_run;
-            sm_l[wave * 16 + c] = l_run;
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < DB / 4; ++q)
+                    my_o[(i * (DB / 4) + q) * 64 + lane] =
+                        make_float4(acc[h][4 * q][i], acc[h][4 * q + 1][i], acc[h][4 * q + 2][i], acc[h][4 * q + 3][i]);
+            if (a == 0) {
+                sm_m[(wave * NH + h) * 16 + c] = m_run[h];
+                sm_l[(wave * NH + h) * 16 + c] = l_run[h];
+            }
         }
     }
     __syncthreads();
     if (live) {
-        const int hq = head0 + c;
-        float lse_nat = 0.f;
-        auto merge = [&](auto share_tag) {
+        auto merge = [&](auto share_tag, int h) {
             constexpr int TI = decltype(share_tag)::value;
+            const int hq = head0 + h * p.group + c;
+            const int64_t prow = prow0 + h * kv_step + (int64_t)c * prow_step;
             float mw[TI], lw[TI];
             float mx = -INFINITY;
 #pragma unroll
             for (int t = 0; t < TI; ++t) {
-                mw[t] = sm_m[t * 16 + c];
-                lw[t] = sm_l[t * 16 + c];
+                mw[t] = sm_m[(t * NH + h) * 16 + c];
+                lw[t] = sm_l[(t * NH + h) * 16 + c];
                 mx = fmaxf(mx, mw[t]);
             }
             float sc[TI], l = 0.f;
@@ -372,13 +473,13 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
                 l += lw[t] * sc[t];
             }
             const float norm = fast_rcp(l);
-            lse_nat = (mx + fast_log2(l)) * kLn2;
+            const float lse_nat = (mx + fast_log2(l)) * kLn2;
 #pragma unroll
             for (int t = 0; t < TI; ++t) sc[t] *= norm;
             for (int e = wave; e < DB; e += TI) {
                 float4 xw[TI];
 #pragma unroll
-                for (int t = 0; t < TI; ++t) xw[t] = reinterpret_cast<const float4*>(lds + t * kScratch)[e * 64 + lane];
+                for (int t = 0; t < TI; ++t) xw[t] = reinterpret_cast<const float4*>(lds + (t * NH + h) * kScratch)[e * 64 + lane];
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int t = 0; t < TI; ++t) {
@@ -389,19 +490,19 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
                 }
                 const int d0 = DB * (4 * a + e / (DB / 4)) + 4 * (e % (DB / 4));
                 if (p.direct) store_out4(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + d0, o, p.out_dtype);
-                else *reinterpret_cast<float4*>(p.part_o + (prow0 + (int64_t)c * prow_step) * DV + d0) = o;
+                else *reinterpret_cast<float4*>(p.part_o + prow * DV + d0) = o;
+            }
+            if (wave == 0 && a == 0) {
+                if (p.direct) {
+                    if (p.lse) p.lse[(int64_t)b * p.lse_sb + hq] = lse_nat;
+                    if (p.pack_lse) store_out(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + DV, lse_nat, p.out_dtype);
+                } else {
+                    p.part_lse[prow] = lse_nat;
+                }
             }
         };
-        if (nw == 8) merge(IntTag<8>());
-        else merge(IntTag<4>());
-        if (wave == 0 && a == 0) {
-            if (p.direct) {
-                if (p.lse) p.lse[(int64_t)b * p.lse_sb + hq] = lse_nat;
-                if (p.pack_lse) store_out(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + DV, lse_nat, p.out_dtype);
-            } else {
-                p.part_lse[prow0 + (int64_t)c * prow_step] = lse_nat;
-            }
-        }
+#pragma unroll
+        for (int h = 0; h < NH; ++h) merge(IntTag<kWaves>(), h);
     }
     };   // run_piece
 #include "fdk_splitkv_mfma_work.h"
@@ -411,34 +512,50 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
 template <int QDT, int D>
 int launch_mx4(const SplitParams& p_in, const Mx4Scales& x, hipStream_t stream) {
     SplitParams p = p_in;
-    if (p.fused || p.probe || p.hg_per_wg != 1) return (int)hipErrorInvalidValue;
+    if (p.fused || p.probe || p.hkv % p.hg_per_wg) return (int)hipErrorInvalidValue;
     p.head_tiles = (p.group + 15) / 16;
-    p.hg_blocks = p.hkv;
+    p.hg_blocks = p.hkv / p.hg_per_wg;
     p.persistent = 0;
     const unsigned units = (unsigned)(p.hg_blocks * p.head_tiles);
     const dim3 grid = p.balanced ? dim3(units, (unsigned)p.workgroups / units) : dim3(units, (unsigned)p.num_splits, (unsigned)p.batch);
     p.shares = (int32_t)grid.y;
     p.grid_x = (int32_t)grid.x;
-    const int nw = 8;
-    p.wavefronts = nw;
-    const size_t lds_bytes = (size_t)nw * (D * 64 + 2 * 16 * sizeof(float)) + 16;
-    const int pm = (p.page_shift >= 0 && p.page_size % 16 == 0) ? PM_TILE : PM_ROW;
-#define FDK_MX4_LAUNCH(PMV, MODEV)                                                                                            \
-    do {                                                                                                                      \
-        if (lds_bytes > 64 * 1024) {                                                                                          \
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&splitkv_mx4_kernel<QDT, PMV, D, MODEV>),  \
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes);             \
-            if (e != hipSuccess) return (int)e;                                                                               \
-        }                                                                                                                     \
-        hipLaunchKernelGGL((splitkv_mx4_kernel<QDT, PMV, D, MODEV>), grid, dim3(64 * nw), lds_bytes, stream, p, x);           \
+    p.wavefronts = kWaves;
+    const size_t lds_bytes = (size_t)kWaves * p.hg_per_wg * (D * 64 + 2 * 16 * sizeof(float)) + 16;
+    const bool tile = p.page_shift >= 0 && p.page_size % 16 == 0;
+#define FDK_MX4_LAUNCH(PMV, MODEV, NHV, STV)                                                                                           \
+    do {                                                                                                                               \
+        if (lds_bytes > 64 * 1024) {                                                                                                   \
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&splitkv_mx4_kernel<QDT, PMV, D, MODEV, NHV, STV>), \
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes);                      \
+            if (e != hipSuccess) return (int)e;                                                                                        \
+        }                                                                                                                              \
+        hipLaunchKernelGGL((splitkv_mx4_kernel<QDT, PMV, D, MODEV, NHV, STV>), grid, dim3(64 * kWaves), lds_bytes, stream, p, x);      \
     } while (0)
-    if (p.balanced) {
-        if (pm == PM_TILE) FDK_MX4_LAUNCH(PM_TILE, WM_SHARES);
-        else FDK_MX4_LAUNCH(PM_ROW, WM_SHARES);
+#define FDK_MX4_LAUNCH_NH(NHV, STV)                                 \
+    do {                                                            \
+        if (p.balanced) {                                           \
+            if (tile) FDK_MX4_LAUNCH(PM_TILE, WM_SHARES, NHV, STV); \
+            else FDK_MX4_LAUNCH(PM_ROW, WM_SHARES, NHV, STV);       \
+        } else {                                                    \
+            if (tile) FDK_MX4_LAUNCH(PM_TILE, WM_ONE, NHV, STV);    \
+            else FDK_MX4_LAUNCH(PM_ROW, WM_ONE, NHV, STV);          \
+        }                                                           \
+    } while (0)
+    // Lines that no other workgroup reads: one q-head tile, and rows of whole lines or no neighbour within the line
+    const bool stream_rows = p.head_tiles == 1 && (D >= 256 || p.hkv == 1 || (p.k_sh > D / 2 && p.v_sh > D / 2));
+    if (p.hg_per_wg == 1) {
+        if (stream_rows) FDK_MX4_LAUNCH_NH(1, true);
+        else FDK_MX4_LAUNCH_NH(1, false);
     } else {
-        if (pm == PM_TILE) FDK_MX4_LAUNCH(PM_TILE, WM_ONE);
-        else FDK_MX4_LAUNCH(PM_ROW, WM_ONE);
+        if constexpr (D <= 128) {
+            if (p.hg_per_wg != 2) return (int)hipErrorInvalidValue;
+            FDK_MX4_LAUNCH_NH(2, false);
+        } else {
+            return (int)hipErrorInvalidValue;
+        }
     }
+#undef FDK_MX4_LAUNCH_NH
 #undef FDK_MX4_LAUNCH
     return (int)hipGetLastError();
 }

@@ -102,10 +102,14 @@ class PagedKVCache:
         # (one allocation for both pools, the V pool 256 bytes off the K pool modulo 512: see alloc_kv_pools)
         self.k_block_scale = self.v_block_scale = None
         if self.mxfp4:
-            k, v = alloc_kv_pools(shape[:3] + (head_dim // 2,), torch.uint8, self.device, zero=True)
-            self.key_cache, self.value_cache = k.view(dtype), v.view(dtype)
-            self.k_block_scale = torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.uint8, device=self.device)
-            self.v_block_scale = torch.zeros_like(self.k_block_scale)
+            # In memory [num_blocks, Hkv, PAGE_SIZE, ...]: a row is half a 128-byte line or less, and a decode workgroup, which
+            # reads one kv head, then finds its rows side by side instead of sharing every line with the neighbouring head's
+            # (4 sequences x 8 kv heads x 131072 tokens: 93 us against 116 us).
+            by_head = (num_blocks, num_kv_heads, PAGE_SIZE)
+            k, v = alloc_kv_pools(by_head + (head_dim // 2,), torch.uint8, self.device, zero=True)
+            self.key_cache, self.value_cache = k.view(dtype).transpose(1, 2), v.view(dtype).transpose(1, 2)
+            self.k_block_scale, self.v_block_scale = (
+                torch.zeros(by_head + (head_dim // 32,), dtype=torch.uint8, device=self.device).transpose(1, 2) for _ in range(2))
         else:
             self.key_cache, self.value_cache = alloc_kv_pools(shape, dtype, self.device, zero=True)
         if fill == "randn":
