@@ -31,6 +31,7 @@ def _args(**kw):
     a.sm_scale = 0.088
     a.out_stride_b, a.out_stride_h, a.lse_stride_b = 32 * 128, 128, 32
     a.max_kv_len = a.min_kv_len = 4096
+    a.workspace, a.workspace_bytes = 0xA0000, 1 << 40
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -74,18 +75,25 @@ def test_a_caller_of_the_previous_revision_is_asked_for_scales():
 
 
 def test_plans():
-    """Every plan takes one kv head per workgroup; a batch that fills the compute units alone is a single pass, short ones
-    are cut into chunks, long ragged ones into equal shares."""
+    """Two kv heads per workgroup where their rows share lines (heads side by side, rows below 128 bytes), unless only one each
+    fills the compute units; short batches are cut into chunks, long ragged ones into equal shares."""
     plan = FdkPlan()
     lib = _lib.load()
-    assert lib.fdk_plan(C.byref(_args()), 0, C.byref(plan)) == 0
-    assert (plan.num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 1, 0)
+
+    def of(**kw):
+        assert lib.fdk_plan(C.byref(_args(**kw)), 0, C.byref(plan)) == 0
+        assert plan.algo == _lib.FDK_ALGO_MFMA and (not plan.balanced or plan.workgroups % (8 // plan.kv_heads_per_wg) == 0)
+        return plan
+    assert (of().num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 1, 0)
+    assert (of(batch=64).num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 2, 0)
+    by_head = dict(k_stride_head=16 * 64, k_stride_tok=64, v_stride_head=16 * 64, v_stride_tok=64)
+    assert of(batch=64, **by_head).kv_heads_per_wg == 1
+    wide = dict(head_dim=256, k_stride_head=128, v_stride_head=128, k_stride_tok=1024, v_stride_tok=1024)
+    assert of(batch=64, **wide).kv_heads_per_wg == 1
+    assert of(batch=64, num_kv_heads=1, num_q_heads=8).kv_heads_per_wg == 1
     for kw in (dict(batch=2), dict(batch=3, min_kv_len=0), dict(batch=40, min_kv_len=0, max_kv_len=0, max_pages=8192, table_stride_b=8192),
                dict(batch=4, max_pages=16384, table_stride_b=16384, max_kv_len=0, min_kv_len=0)):
-        assert lib.fdk_plan(C.byref(_args(**kw)), 0, C.byref(plan)) == 0
-        assert plan.kv_heads_per_wg == 1 and plan.algo == _lib.FDK_ALGO_MFMA
-        assert plan.num_splits > 1
-        assert not plan.balanced or plan.workgroups % 8 == 0
+        assert of(**kw).num_splits > 1
 
 
 def _conv(**kw):

@@ -286,9 +286,13 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
     return FDK_OK;
 }
 
-int mx_kv_heads_per_wg(const fdk_decode_args* a) {
+// kv heads per workgroup of the MXFP4 kernels: two where rows of neighbouring heads are parts of the same 128-byte lines, so that
+// one compute unit reads whole lines - unless only single heads give every compute unit a workgroup, and with it a single pass:
+// the combine launch then costs what the whole lines save (batch 32 x 8 kv heads x 4096 tokens: 36 us either way).
+int mx_kv_heads_per_wg(const fdk_decode_args* a, int64_t head_units, int num_cus) {
     const bool neighbours = a->k_stride_head == a->head_dim / 2 && a->v_stride_head == a->head_dim / 2;
-    return neighbours && a->head_dim <= 128 && a->num_kv_heads % 2 == 0 ? 2 : 1;
+    if (!neighbours || a->head_dim > 128 || a->num_kv_heads % 2) return 1;
+    return head_units >= num_cus && head_units / 2 < num_cus ? 1 : 2;
 }
 
 int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
@@ -319,7 +323,7 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
     const int tile_heads = algo == FDK_ALGO_MFMA ? fdk::mfma_heads_per_wg(group, a->head_dim + v_dim(a), a->kv_dtype) : 16;   // q heads of a kv head per workgroup
     if (algo == FDK_ALGO_MFMA) {
         kv_heads_per_wg = a->kv_dtype == FDK_MXFP4
-                              ? mx_kv_heads_per_wg(a)
+                              ? mx_kv_heads_per_wg(a, (int64_t)batch * a->num_kv_heads * ((group + 15) / 16), num_cus)
                               : fdk::mfma_kv_heads_per_wg(batch, a->num_kv_heads, group, num_cus, a->head_dim + v_dim(a), a->kv_dtype);
         units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
     } else {
@@ -361,7 +365,7 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
         if (rebalance) {
             kv_heads_per_wg = a->num_kv_heads % 2 ? 1 : 2;
             if (tile_heads > 16) kv_heads_per_wg = 1;
-            if (a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = mx_kv_heads_per_wg(a);
+            if (a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = mx_kv_heads_per_wg(a, 0, num_cus);
             units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
         }
     }
