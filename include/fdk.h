@@ -484,7 +484,7 @@ int fdk_accumulate_weights(const fdk_attn_weights_args* args, void* hip_stream);
 
 /* Evict the tokens of least weight (see fdk_kv_evict_args).  Calls that overlap in time need distinct workspaces. */
 int fdk_kv_evict(const fdk_kv_evict_args* args, void* hip_stream);
-size_t fdk_kv_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads);
+size_t fdk_kv_evict_workspace_bytes(const fdk_kv_evict_args* args); /* (reads sizes only; for the current device) */
 
 #ifdef __cplusplus
 }

@@ -178,6 +178,42 @@ def test_long_rows_and_many_sequences(cuda_device, kind, batch, keep):
     _evict(kind, lens, 2 if batch == 1 else 8, 64, 16, keep, 100, torch.bfloat16, 5, cuda_device, in_place=batch > 1)
 
 
+@pytest.mark.parametrize("b,hkv,length,keep,recent,d", [(1, 1, 70000, 9000, 100, 64), (1, 3, 40000, 39000, 0, 64), (4, 16, 60000, 5000, 5000, 64),
+                                                        (4, 16, 60000, 3000, 17, 64), (2, 100, 90000, 700, 10, 32), (1, 1, 270000, 1000, 500, 32)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rows_spread_over_workgroups(cuda_device, b, hkv, length, keep, recent, d, in_place):
+    """Long rows, whose weights several workgroups share: a few of them, many, and so many that each holds its weights in
+    registers no more; ragged lengths with one that needs no eviction.  Against a stable sort."""
+    import triton_distributed_amd as tda
+    dev = cuda_device
+    g = torch.Generator(device=dev).manual_seed(length + hkv)
+    page, per = 64, (length + 63) // 64
+    table = torch.randperm(b * per, generator=g, device=dev).to(torch.int32).view(b, per)
+    k = torch.randint(0, 256, (b * per, page, hkv, d), generator=g, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    v = torch.randint(0, 256, (b * per, page, hkv, d), generator=g, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    lens = torch.tensor([length, keep - 1, keep + 1, length // 2][:b], dtype=torch.int32, device=dev)
+    w = (torch.rand(b, hkv, length, generator=g, device=dev) ** 8 * 1000).round() / 8                  # many zeros, many ties
+    w[0, 0] = w[0, 0, 0]                                                                              # a row of equal weights
+    want_k, want_v, want_w = k.view(torch.uint8).clone(), v.view(torch.uint8).clone(), torch.zeros_like(w)
+    want_kept = torch.full((b, hkv, keep), -1, dtype=torch.int32, device=dev)
+    for i, n in enumerate(lens.tolist()):
+        order = w[i, :, :n].clone()
+        order[:, max(n - recent, 0):] = math.inf
+        stay = torch.sort(order, dim=-1, descending=True, stable=True).indices[:, :keep].sort(-1).values
+        m = stay.shape[1]
+        want_kept[i, :, :m] = stay.to(torch.int32)
+        want_w[i, :, :m] = w[i].gather(-1, stay)
+        head, to = torch.arange(hkv, device=dev)[:, None], torch.arange(m, device=dev)
+        row = table[i].long()
+        for pool in (want_k, want_v):
+            pool[row[to // page], to % page, head] = pool[row[stay // page], stay % page, head]
+    new, kept, wo = tda.evict_kvcache(k, v, table, lens, w, keep, recent, weights_out=w if in_place else None)
+    assert torch.equal(kept, want_kept)
+    assert torch.equal(wo, want_w) and (wo.data_ptr() == w.data_ptr()) == in_place
+    assert torch.equal(new, lens.clamp(max=keep))
+    assert torch.equal(k.view(torch.uint8), want_k) and torch.equal(v.view(torch.uint8), want_v)
+
+
 def test_weights_that_order_awkwardly(cuda_device):
     """All alike, all zero, both zeros, negative, infinite, NaN, subnormal, apart in the last bit only."""
     n = 400

@@ -78,6 +78,20 @@ def test_evict_refusals(kw, code):
     assert _lib.load().fdk_kv_evict(C.byref(_evict_args(**kw)), None) == code, _lib.load().fdk_last_error()
 
 
+def test_workspace_of_long_rows():
+    """One plan entry a row; rows that few workgroups would have to themselves need room for counts and weights."""
+    lib = _lib.load()
+    of = lambda **kw: lib.fdk_kv_evict_workspace_bytes(C.byref(_evict_args(**kw)))
+    assert of() == 32 * 8 * 16
+    long = dict(batch=1, max_pages=4096, table_stride_b=4096, weights_len=65536, weights_stride_h=65536, weights_out_stride_h=65536)
+    need = of(**long)
+    assert need > 8 * 2048 * 4 and of(**dict(long, keep=4096)) == need + 8 * 2048 * 4
+    assert lib.fdk_kv_evict(C.byref(_evict_args(**dict(long, workspace_bytes=need - 1))), None) == _lib.FDK_EWORKSPACE
+    assert lib.fdk_kv_evict(C.byref(_evict_args(**dict(long, workspace_bytes=need))), None) == 0
+    assert of(batch=0) == 0 and of(struct_size=4) == 0 and of(max_pages=1 << 30) == 0
+    assert lib.fdk_kv_evict_workspace_bytes(None) == 0
+
+
 def test_python_refusals():
     k = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
     table, n, w = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 2, 64)

@@ -228,7 +228,7 @@ def load() -> C.CDLL:
     lib.fdk_kv_evict.restype = C.c_int
     lib.fdk_kv_evict.argtypes = [C.POINTER(FdkKvEvictArgs), C.c_void_p]
     lib.fdk_kv_evict_workspace_bytes.restype = C.c_size_t
-    lib.fdk_kv_evict_workspace_bytes.argtypes = [C.c_int32, C.c_int32]
+    lib.fdk_kv_evict_workspace_bytes.argtypes = [C.POINTER(FdkKvEvictArgs)]
     for name in ("fdk_mx_quantize", "fdk_mx_dequantize"):
         fn = getattr(lib, name)
         fn.restype = C.c_int

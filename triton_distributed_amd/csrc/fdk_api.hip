@@ -1087,9 +1087,16 @@ int fdk_accumulate_weights(const fdk_attn_weights_args* caller_args, void* hip_s
     return FDK_OK;
 }
 
-size_t fdk_kv_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads) {
-    if (batch <= 0 || num_kv_heads <= 0) return 0;
-    return (size_t)batch * (size_t)num_kv_heads * 16;
+static int evict_max_tokens(const fdk_kv_evict_args* a) {
+    return a->max_pages * a->page_size < a->weights_len ? a->max_pages * a->page_size : a->weights_len;
+}
+
+size_t fdk_kv_evict_workspace_bytes(const fdk_kv_evict_args* a) {
+    if (!a || a->struct_size < sizeof(fdk_kv_evict_args) || a->batch <= 0 || a->num_kv_heads <= 0 || a->weights_len <= 0 || a->keep <= 0 ||
+        a->page_size <= 0 || a->max_pages <= 0 || (int64_t)a->max_pages * a->page_size > kMaxTableTokens)
+        return 0;
+    const int cus = a->flags & FDK_FLAG_DRY_RUN ? kDryRunCus : query_cus();
+    return fdk::evict_workspace_bytes(a->batch, a->num_kv_heads, evict_max_tokens(a), a->keep, cus);
 }
 
 int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
@@ -1134,7 +1141,7 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     if (a->weights == a->weights_out &&
         ((a->num_kv_heads > 1 && a->weights_stride_h != a->weights_out_stride_h) || (a->batch > 1 && a->weights_stride_b != a->weights_out_stride_b)))
         return fail(FDK_ESHAPE, "weights_out may be weights itself only with its strides");
-    const size_t need = fdk_kv_evict_workspace_bytes(a->batch, a->num_kv_heads);
+    const size_t need = fdk_kv_evict_workspace_bytes(a);
     if (!a->workspace || a->workspace_bytes < need) return fail(FDK_EWORKSPACE, "workspace has %zu bytes; %zu needed", a->workspace ? a->workspace_bytes : 0, need);
     if (!aligned16(a->workspace)) return fail(FDK_EALIGN, "workspace must be 16-byte aligned");
     if (a->flags & FDK_FLAG_DRY_RUN) return FDK_OK;
@@ -1155,7 +1162,7 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     p.wo_sb = a->weights_out_stride_b; p.wo_sh = a->weights_out_stride_h;
     p.batch = a->batch; p.hkv = a->num_kv_heads; p.keep = a->keep; p.recent = a->recent;
     p.weights_len = a->weights_len;
-    p.max_tokens = a->max_pages * a->page_size < a->weights_len ? a->max_pages * a->page_size : a->weights_len;
+    p.max_tokens = evict_max_tokens(a);
     p.page_size = a->page_size; p.page_shift = ilog2_exact(a->page_size);
     const int rc = fdk::launch_kv_evict(p, query_cus(), reinterpret_cast<hipStream_t>(hip_stream));
     if (rc) return fail(rc, "eviction launch failed: %s", hipGetErrorString((hipError_t)rc));

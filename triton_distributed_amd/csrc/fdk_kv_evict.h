@@ -49,9 +49,17 @@ struct EvictParams {
     int32_t weights_len, max_tokens;
     int32_t page_size, page_shift;
     int32_t num_tensors;
+    // rows whose weights are spread over several workgroups (parts of the workspace)
+    int32_t segments;
+    int2* row_state;                         // [rows][2]: leading bits of the last survivor's weight, survivors left to find
+    int32_t* seg_gt;                         // [rows][segments]: weights known to be above them
+    uint16_t* seg_hist;                      // [3][rows][segments][2048]
+    float* stash;                            // [rows][keep]: the survivors' weights
 };
 
 int launch_attn_weights(const AttnWeightsParams& p, int head_dim, int q_dtype, int kv_dtype, int num_cus, hipStream_t stream);
+int evict_segments(int batch, int hkv, int max_tokens, int num_cus);
+size_t evict_workspace_bytes(int batch, int hkv, int max_tokens, int keep, int num_cus);
 int launch_kv_evict(const EvictParams& p, int num_cus, hipStream_t stream);
 
 }  // namespace fdk

@@ -116,17 +116,15 @@ def accumulate_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, block_t
 _EVICT_TEMPLATES = {}
 
 
-def _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept):
+def _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept, workspace_bytes):
     batch, kv_heads = weights.shape[:2]
     if weights_out is None:
         weights_out = torch.empty(weights.shape, dtype=torch.float32, device=weights.device)
     if kv_lens_out is None:
         kv_lens_out = torch.empty(kv_lens.shape, dtype=torch.int32, device=weights.device)
-    # (one allocation for the indices and, 16-byte aligned in front of them, the workspace)
-    head = batch * kv_heads * 4
-    buf = torch.empty(head + (0 if kept is not None else batch * kv_heads * keep), dtype=torch.int32, device=weights.device)
     if kept is None:
-        kept = buf[head:].view(batch, kv_heads, keep)
+        kept = torch.empty((batch, kv_heads, keep), dtype=torch.int32, device=weights.device)
+    buf = torch.empty(workspace_bytes, dtype=torch.uint8, device=weights.device)
     return weights_out, kv_lens_out, kept, buf
 
 
@@ -193,13 +191,13 @@ def evict_kvcache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tabl
         a.batch, a.num_kv_heads, a.head_dim, a.v_head_dim = batch, kv_heads, _row_values(key_cache), _row_values(value_cache)
         a.page_size, a.max_pages, a.weights_len = key_cache.shape[1], block_table.shape[1], length
         a.keep, a.recent = keep, recent
-        a.workspace_bytes = _LIB.fdk_kv_evict_workspace_bytes(batch, kv_heads)
+        a.workspace_bytes = _LIB.fdk_kv_evict_workspace_bytes(C.byref(a))
     if stream is None:
-        weights_out, kv_lens_out, kept, buf = _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept)
+        weights_out, kv_lens_out, kept, buf = _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept, a.workspace_bytes)
     else:
         # (the kernels run on that stream: the workspace must go back to its pool, not to the current stream's)
         with _on_stream(weights.device, _stream_handle(stream)):
-            weights_out, kv_lens_out, kept, buf = _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept)
+            weights_out, kv_lens_out, kept, buf = _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept, a.workspace_bytes)
     a.weights_out_stride_b, a.weights_out_stride_h = weights_out.stride(0), weights_out.stride(1)
     a.k_cache, a.v_cache = key_cache.data_ptr(), value_cache.data_ptr()
     if k_scale is not None:
