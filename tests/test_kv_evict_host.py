@@ -41,6 +41,7 @@ MX = dict(kv_dtype=_lib.FDK_MXFP4, k_stride_page=16 * 8 * 64, k_stride_tok=8 * 6
     (dict(lse_stride_b=31), _lib.FDK_ESHAPE), (dict(page_size=0), _lib.FDK_ESHAPE), (dict(max_pages=1 << 27), _lib.FDK_ESHAPE),
     (dict(table_stride_b=255), _lib.FDK_ESHAPE), (dict(sm_scale=math.inf), _lib.FDK_ESHAPE), (dict(soft_cap=math.nan), _lib.FDK_ESHAPE),
     (dict(k_stride_head=120), _lib.FDK_ESHAPE), (dict(batch=70000), _lib.FDK_ESHAPE), (dict(MX, kbs_stride_head=3), _lib.FDK_ESHAPE),
+    (dict(k_stride_page=1 << 31), _lib.FDK_ESHAPE), (dict(k_stride_tok=1 << 27), _lib.FDK_ESHAPE),
 ])
 def test_weights_refusals(kw, code):
     assert _lib.load().fdk_accumulate_weights(C.byref(_weights_args(**kw)), None) == code, _lib.load().fdk_last_error()

@@ -1052,6 +1052,9 @@ int fdk_accumulate_weights(const fdk_attn_weights_args* caller_args, void* hip_s
     if (int rc = check_pages(a->batch, a->page_size, a->max_pages, a->table_stride_b, a->block_table, a->kv_lens)) return rc;
     const int es = elem_size(a->kv_dtype), row_bytes = mx ? d / 2 : d * es;
     if (int rc = check_rows("k_cache", a->k_cache, a->k_stride_page, a->k_stride_tok, a->k_stride_head, es, row_bytes, a->num_kv_heads)) return rc;
+    if (a->k_stride_page * es >= ((int64_t)1 << 32) || a->k_stride_tok * es >= ((int64_t)1 << 28) ||
+        a->page_size * (a->k_stride_tok * es) >= ((int64_t)1 << 32))
+        return fail(FDK_ESHAPE, "cache strides too large: a page must span less than 4 GiB");
     if (!a->q || !a->lse || !a->weights) return fail(FDK_ENULL, "q / lse / weights must be non-null");
     if (!aligned16(a->q) || a->q_stride_b % 8 || a->q_stride_h % 8) return fail(FDK_EALIGN, "q and its strides must be 16-byte aligned");
     if ((reinterpret_cast<uintptr_t>(a->lse) | reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->k_scale)) & 3u)

@@ -4,8 +4,8 @@
 // One pass over the K rows, no softmax of its own: the logits of 16 tokens x 16 q heads are S = Q K^T by MFMA with both
 // operands loaded straight in their layouts, K as operand B (lane (c, a): token c, its a-th piece of every 64 bytes), so that
 // lane (c, a) holds token c's logits of heads 4a .. 4a + 3 and the sum over the heads is three additions and two exchanges.
-// Every weight belongs to one wavefront: no atomics, the same bits on every run.  A workgroup takes a share of a sequence for
-// one kv head; its wavefronts interleave steps.  Bound by the bytes of the K rows.
+// Every weight belongs to one wavefront: no atomics, the same bits on every run.  Bound by the bytes of the K rows: 32
+// sequences x 8 kv heads x 4096 tokens x 256 bytes in 51 us, 5.4 TB/s (one head a workgroup: 59 us); an fp8 cache 30 us.
 #include "fdk_kv_evict.h"
 
 namespace fdk {
@@ -14,6 +14,9 @@ namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;                  // wavefronts of a workgroup
+constexpr int kWorkgroupsPerCu = 4;
 
 enum KeyKind { KEY_16BIT = 0, KEY_FP8 = 1, KEY_MX4 = 2 };
 
@@ -44,20 +47,27 @@ __device__ __forceinline__ constexpr int first_value(int step, int a) {
 }
 
 // MANY: more than 16 q heads per kv head - their fragments are read again for every step (from the L1) instead of being held
-template <int QDT, int KIND, int D, bool MANY>
-__global__ __launch_bounds__(256) void attn_weights_kernel(const AttnWeightsParams p) {
+// TILE: pages of a power of two and at least 16 tokens - one page number per tile of 16, wave-uniform addresses
+template <int QDT, int KIND, int D, bool MANY, bool TILE>
+__global__ __launch_bounds__(64 * kWaves) void attn_weights_kernel(const AttnWeightsParams p) {
     using P2 = Pack2<QDT>;
     constexpr int STEPS = D / 32;
-    constexpr int TILES = D <= 128 ? 2 : 1;                // tiles of 16 tokens whose rows are under way together
+    // tiles of 16 tokens whose rows are under way together (four, where rows are short, measured 30-40 % slower: the shares of
+    // ragged batches are cut into longer steps)
+    constexpr int TILES = KIND == KEY_16BIT ? (D <= 128 ? 2 : 1) : KIND == KEY_FP8 ? (D <= 256 ? 2 : 1) : 2;
+    constexpr bool kWholeLines = (KIND == KEY_16BIT ? 2 * D : KIND == KEY_FP8 ? D : D / 2) % 128 == 0;
     constexpr int LOADS = KIND == KEY_16BIT ? STEPS : KIND == KEY_FP8 ? D / 64 : D > 64 ? D / 128 : 1;     // 16-byte pieces
     constexpr int MXS = KIND == KEY_MX4 && D == 256 ? 2 : 1;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int a = lane >> 4, c = lane & 15;
-    // rows of less than 128 bytes share cache lines with the neighbouring heads': all heads of a (sequence, share) on one XCD
+    // A unit of work: a share of a sequence for a block of nh neighbouring kv heads, one to a wavefront (the wavefronts of a head
+    // interleave steps): together they read longer runs of every token, and rows below 128 bytes share their lines within the
+    // workgroup; all blocks of a (sequence, share) run on one XCD, whose L2 then serves what blocks share.
+    const int nh = p.heads_per_wg, blocks = p.hkv / nh;
     int unit, row;
     {
-        const int id = (int)blockIdx.x, rows = p.batch * p.shares, T = p.hkv;
+        const int id = (int)blockIdx.x, rows = p.batch * p.shares, T = blocks;
         const int full = rows & ~7;
         if (id < full * T) {
             const int blk = id / (8 * T), in = id - blk * 8 * T;
@@ -69,15 +79,8 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(const AttnWeightsPara
             unit = rest % T;
         }
     }
-    const int kvh = unit, b = row / p.shares, share = row - b * p.shares;
-    const int kv_len = min(p.kv_lens[b], p.max_tokens);
-    constexpr int kWgStep = 4 * 16 * TILES;
-    // equal shares of the sequence's own length
-    const int per = max(((kv_len + p.shares - 1) / p.shares + kWgStep - 1) / kWgStep, 1) * kWgStep;
-    const int64_t begin64 = (int64_t)share * per;
-    if (begin64 >= kv_len) return;
-    const int begin = (int)begin64, end = (int)min(begin64 + per, (int64_t)kv_len);
-
+    const int kvh = unit * nh + wave % nh, b = row / p.shares, share = row - b * p.shares;
+    // (what does not depend on the length is requested before it)
     const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb;
     const float* lse_row = p.lse + (int64_t)b * p.lse_sb;
     const int head_tiles = MANY ? (p.group + 15) / 16 : 1;
@@ -91,8 +94,17 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(const AttnWeightsPara
         for (int i = 0; i < 4; ++i) lse2[i] = lse_row[kvh * p.group + min(ht * 16 + 4 * a + i, p.group - 1)] * kLog2e;
     };
     if (!MANY) load_q(0);
+    typedef const __attribute__((address_space(4))) int32_t* ConstI32;     // read-only for the whole kernel: scalar loads
+    const int kv_len = min(((ConstI32)(uintptr_t)p.kv_lens)[b], p.max_tokens);
+    const int wg_step = kWaves / nh * 16 * TILES;
+    // equal shares of the sequence's own length
+    const int per = max(((kv_len + p.shares - 1) / p.shares + wg_step - 1) / wg_step, 1) * wg_step;
+    const int64_t begin64 = (int64_t)share * per;
+    if (begin64 >= kv_len) return;
+    const int begin = (int)begin64, end = (int)min(begin64 + per, (int64_t)kv_len);
 
-    const int32_t* tbl = p.block_table + (int64_t)b * p.tbl_sb;
+
+    const ConstI32 tbl = (ConstI32)(uintptr_t)(p.block_table + (int64_t)b * p.tbl_sb);
     const char* kplane = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh;
     const uint8_t* splane = p.k_block_scale + (int64_t)kvh * p.bs_sh;
     float* wrow = p.weights + (int64_t)b * p.w_sb + (int64_t)kvh * p.w_sh;
@@ -102,62 +114,78 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(const AttnWeightsPara
     const float inv_cap = softcap ? 1.0f / p.soft_cap : 0.f;
 
     auto page_of = [&](int n) { return tbl[p.page_shift < 0 ? n / p.page_size : n >> p.page_shift]; };
-    int32_t pg[TILES];
-    int tok = begin + wave * 16 * TILES;
-    if (tok >= end) return;
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) pg[t] = page_of(min(tok + 16 * t + c, end - 1));
-    for (; tok < end; tok += kWgStep) {
-        // rows past the end repeat the last one
+    struct Step {
         uint4 raw[TILES][LOADS];
         uint32_t sc[TILES][MXS];
+        float old;
+    };
+    struct Pages { int32_t pg[TILES]; };
+    // (positions past the end: the last token's page)
+    auto first_of = [&](int tok, int t) { return min(tok + 16 * t, (end - 1) & ~15); };       // TILE
+    auto fetch_pages = [&](int tok, Pages& pi) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+            pi.pg[t] = TILE ? tbl[first_of(tok, t) >> p.page_shift] : page_of(min(tok + 16 * t + c, end - 1));
+    };
+    // byte offset of a row: page strides and in-page offsets are below 4 GiB, one 32 x 32 -> 64 bit multiply-add
+    auto offset = [&](int64_t sp, int64_t st, uint32_t pg, uint32_t slot) {
+        return (uint64_t)pg * (uint32_t)sp + (uint64_t)(slot * (uint32_t)st);
+    };
+    // rows past the end repeat the last one; lane 16 t + c keeps the weight of token c of tile t
+    auto issue = [&](int tok, const Pages& pi, Step& r) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            const int n = min(tok + 16 * t + c, end - 1);
-            const int64_t in_page = p.page_shift < 0 ? n % p.page_size : (n & (p.page_size - 1));
-            const char* kp = kplane + (int64_t)pg[t] * p.k_sp + in_page * p.k_st;
+            const char *kp, *sp;
+            if constexpr (TILE) {
+                const int first = first_of(tok, t);
+                const uint32_t slot = (uint32_t)(first & (p.page_size - 1)), mine = (uint32_t)min(c, end - 1 - first);
+                kp = kplane + offset(p.k_sp, p.k_st, (uint32_t)pi.pg[t], slot) + (uint32_t)(mine * (uint32_t)p.k_st);
+                sp = reinterpret_cast<const char*>(splane) + offset(p.bs_sp, p.bs_st, (uint32_t)pi.pg[t], slot) + (uint32_t)(mine * (uint32_t)p.bs_st);
+            } else {
+                const int n = min(tok + 16 * t + c, end - 1);
+                const uint32_t slot = (uint32_t)(p.page_shift < 0 ? n % p.page_size : (n & (p.page_size - 1)));
+                kp = kplane + offset(p.k_sp, p.k_st, (uint32_t)pi.pg[t], slot);
+                sp = reinterpret_cast<const char*>(splane) + offset(p.bs_sp, p.bs_st, (uint32_t)pi.pg[t], slot);
+            }
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
                 if constexpr (KIND == KEY_MX4 && D == 64) {
                     const uint2 w = *reinterpret_cast<const uint2*>(kp + 8 * a);
-                    raw[t][j] = make_uint4(w.x, w.y, 0, 0);
+                    r.raw[t][j] = make_uint4(w.x, w.y, 0, 0);
                 } else if constexpr (KIND == KEY_MX4) {
-                    raw[t][j] = *reinterpret_cast<const uint4*>(kp + (D / 8) * a + 16 * j);
+                    r.raw[t][j] = *reinterpret_cast<const uint4*>(kp + (D / 8) * a + 16 * j);
                 } else {
-                    raw[t][j] = *reinterpret_cast<const uint4*>(kp + 64 * j + 16 * a);
+                    // (rows of whole lines are read by one wavefront once: past the caches)
+                    const char* at = kp + 64 * j + 16 * a;
+                    r.raw[t][j] = kWholeLines ? load_stream16(at) : *reinterpret_cast<const uint4*>(at);
                 }
             }
             if constexpr (KIND == KEY_MX4) {
-                const uint8_t* sp = splane + (int64_t)pg[t] * p.bs_sp + in_page * p.bs_st + (D / 4) * a / kMxBlock;
 #pragma unroll
-                for (int g = 0; g < MXS; ++g) sc[t][g] = sp[g];
+                for (int g = 0; g < MXS; ++g) r.sc[t][g] = *reinterpret_cast<const uint8_t*>(sp + (D / 4) * a / kMxBlock + g);
             }
         }
-        // lane 16 t + c keeps the weight of token c of tile t
         const int mine = tok + (lane & (16 * TILES - 1));
-        const bool store = lane < 16 * TILES && mine < end;
-        const float old = store ? wrow[mine] : 0.f;
-        const int next = tok + kWgStep;
-        if (next < end) {
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) pg[t] = page_of(min(next + 16 * t + c, end - 1));
-        }
+        r.old = lane < 16 * TILES && mine < end ? wrow[mine] : 0.f;
+    };
+    auto work = [&](int tok, const Step& r) {
         float sum[TILES];
 #pragma unroll
         for (int t = 0; t < TILES; ++t) sum[t] = 0.f;
         for (int ht = 0; ht < head_tiles; ++ht) {
             if (MANY) load_q(ht);
+            f32x4_t s[TILES];
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
-                f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+                s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int st = 0; st < STEPS; ++st) {
                     uint4 kf;
                     if constexpr (KIND == KEY_16BIT) {
-                        kf = raw[t][st];
+                        kf = r.raw[t][st];
                     } else if constexpr (KIND == KEY_FP8) {
                         // (k8 * scale) rounded to the q dtype, as the decode does by default
-                        const uint4 w = raw[t][st / 2];
+                        const uint4 w = r.raw[t][st / 2];
                         const uint32_t two[2] = {st % 2 ? w.z : w.x, st % 2 ? w.w : w.y};
                         uint32_t o[4];
 #pragma unroll
@@ -169,31 +197,87 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(const AttnWeightsPara
                         }
                         kf = make_uint4(o[0], o[1], o[2], o[3]);
                     } else {
-                        const uint4 w4 = raw[t][st / 4];
+                        const uint4 w4 = r.raw[t][st / 4];
                         const uint32_t w = st % 4 == 0 ? w4.x : st % 4 == 1 ? w4.y : st % 4 == 2 ? w4.z : w4.w;
-                        const float f = mx_scale(sc[t][MXS == 2 ? st / 4 : 0]);
+                        const float f = mx_scale(r.sc[t][MXS == 2 ? st / 4 : 0]);
                         kf = make_uint4(mx_unpack2<QDT, 0>(w, f), mx_unpack2<QDT, 1>(w, f), mx_unpack2<QDT, 2>(w, f), mx_unpack2<QDT, 3>(w, f));
                     }
-                    s = mma16<QDT>(qf[st], kf, s);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float l2 = softcap ? soft_cap_fn(s[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e : s[i] * p.scale_log2;
-                    const float e = fast_exp2(l2 - lse2[i]);
-                    sum[t] += ht * 16 + 4 * a + i < p.group ? e : 0.f;
+                    s[t] = mma16<QDT>(qf[st], kf, s[t]);
                 }
             }
+            if (softcap) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][i] = soft_cap_fn(s[t][i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e;
+            } else {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) s[t] *= p.scale_log2;
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = fast_exp2(s[t][i] - lse2[i]);
+                    sum[t] += ht * 16 + 4 * a + i < p.group ? e : 0.f;
+                }
         }
 #pragma unroll
         for (int t = 0; t < TILES; ++t) sum[t] = sum_across_rows(sum[t]);
-        if (store) wrow[mine] = old + (TILES == 2 && a == 1 ? sum[TILES - 1] : sum[0]);
+        const int mine = tok + (lane & (16 * TILES - 1));
+        if (lane < 16 * TILES && mine < end) {
+            float x = sum[0];
+            if (TILES >= 2 && a == 1) x = sum[TILES >= 2 ? 1 : 0];
+            if (TILES == 4 && a == 2) x = sum[TILES == 4 ? 2 : 0];
+            if (TILES == 4 && a == 3) x = sum[TILES == 4 ? 3 : 0];
+            wrow[mine] = r.old + x;
+        }
+    };
+    // two register buffers (long rows: one): the next step's rows are requested before a step is worked on, page numbers a step
+    // further ahead
+    int tok = begin + wave / nh * 16 * TILES;
+    if (tok >= end) return;
+    Pages pa, pb;
+    fetch_pages(tok, pa);
+    if constexpr (D <= 256) {
+        Step ra, rb;
+        fetch_pages(tok + wg_step, pb);
+        issue(tok, pa, ra);
+        for (;;) {
+            const int next = tok + wg_step, after = next + wg_step;
+            fetch_pages(after, pa);
+            if (next < end) issue(next, pb, rb);
+            work(tok, ra);
+            if (next >= end) return;
+            fetch_pages(after + wg_step, pb);
+            if (after < end) issue(after, pa, ra);
+            work(next, rb);
+            if (after >= end) return;
+            tok = after;
+        }
+    } else {
+        Step r;
+        for (; tok < end; tok += wg_step) {
+            issue(tok, pa, r);
+            fetch_pages(tok + wg_step, pa);
+            work(tok, r);
+        }
     }
 }
 
 template <int QDT, int KIND, int D>
 int launch_d(const AttnWeightsParams& p, dim3 grid, hipStream_t stream) {
-    if (p.group > 16) hipLaunchKernelGGL((attn_weights_kernel<QDT, KIND, D, true>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((attn_weights_kernel<QDT, KIND, D, false>), grid, dim3(256), 0, stream, p);
+    const bool tile = p.page_shift >= 4;
+#define FDK_WEIGHTS_LAUNCH(MANY, TILE) \
+    hipLaunchKernelGGL((attn_weights_kernel<QDT, KIND, D, MANY, TILE>), grid, dim3(64 * kWaves), 0, stream, p)
+    if (p.group > 16) {
+        if (tile) FDK_WEIGHTS_LAUNCH(true, true);
+        else FDK_WEIGHTS_LAUNCH(true, false);
+    } else {
+        if (tile) FDK_WEIGHTS_LAUNCH(false, true);
+        else FDK_WEIGHTS_LAUNCH(false, false);
+    }
+#undef FDK_WEIGHTS_LAUNCH
     return (int)hipGetLastError();
 }
 
@@ -216,11 +300,12 @@ int launch_kind(const AttnWeightsParams& p, int head_dim, dim3 grid, hipStream_t
 
 int launch_attn_weights(const AttnWeightsParams& p_in, int head_dim, int q_dtype, int kv_dtype, int num_cus, hipStream_t stream) {
     AttnWeightsParams p = p_in;
-    // Shares of a sequence per kv head: enough workgroups for eight to a compute unit (they need no merge, so cutting a
-    // sequence finer costs only the loads of q again), at most one per step of 128 tokens.
-    const int64_t units = (int64_t)p.batch * p.hkv;
-    int64_t shares = (8 * (int64_t)num_cus + units - 1) / units;
-    const int64_t most = ((int64_t)p.max_tokens + 127) / 128;
+    p.heads_per_wg = p.hkv % 4 == 0 ? 4 : p.hkv % 2 == 0 ? 2 : 1;
+    // Shares of a sequence per block of heads: enough workgroups for a few to a compute unit (they need no merge, so cutting a
+    // sequence finer costs only the loads of q again), at most one per step.
+    const int64_t units = (int64_t)p.batch * (p.hkv / p.heads_per_wg);
+    int64_t shares = (kWorkgroupsPerCu * (int64_t)num_cus + units - 1) / units;
+    const int64_t most = ((int64_t)p.max_tokens + 31) / 32;
     if (shares > most) shares = most;
     if (shares < 1) shares = 1;
     p.shares = (int32_t)shares;

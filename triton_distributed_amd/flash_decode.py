@@ -981,33 +981,47 @@ def _row_axes(*tensors: torch.Tensor):
     return [m[0] for m in merged], [[m[1 + i] for m in merged] for i in range(len(tensors))]
 
 
+_MXFP4_TEMPLATES = {}          # layout key -> validated argument block without pointers
+
+
 def _mxfp4_convert(fn, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, stream) -> None:
-    d = x.shape[-1]
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"MXFP4 rows are converted from and to bf16 / fp16, not {x.dtype}")
-    if d == 0 or d % MXFP4_BLOCK:
-        raise ValueError(f"rows must hold a multiple of {MXFP4_BLOCK} values, got {d}")
-    if codes.dtype not in _MXFP4_CODES or tuple(codes.shape) != tuple(x.shape[:-1]) + (d // 2,):
-        raise ValueError(f"codes must be uint8 (or float4_e2m1fn_x2) {list(x.shape[:-1]) + [d // 2]}, got {codes.dtype} {list(codes.shape)}")
-    _check_block_scales("scales", scales, codes)
-    for name, t in (("x", x), ("codes", codes)):
-        if not t.is_cuda:
-            raise ValueError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
-        if t.stride(-1) != 1:
-            raise ValueError(f"the last axis of {name} must be contiguous")
-    if x.device != codes.device:
-        raise ValueError(f"codes is on {codes.device}, x on {x.device}")
-    if x.numel() == 0:
-        return
-    n, (xs, cs, ss) = _row_axes(x, codes, scales)
-    a = FdkMxfp4Args()
-    a.struct_size = C.sizeof(FdkMxfp4Args)
+    def meta(t):
+        return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    key = (meta(x), meta(codes), meta(scales))             # (the two directions take the same block)
+    hit = _MXFP4_TEMPLATES.get(key)
+    if hit is not None:
+        a = FdkMxfp4Args.from_buffer_copy(hit)
+    else:
+        d = x.shape[-1]
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"MXFP4 rows are converted from and to bf16 / fp16, not {x.dtype}")
+        if d == 0 or d % MXFP4_BLOCK:
+            raise ValueError(f"rows must hold a multiple of {MXFP4_BLOCK} values, got {d}")
+        if codes.dtype not in _MXFP4_CODES or tuple(codes.shape) != tuple(x.shape[:-1]) + (d // 2,):
+            raise ValueError(f"codes must be uint8 (or float4_e2m1fn_x2) {list(x.shape[:-1]) + [d // 2]}, got {codes.dtype} {list(codes.shape)}")
+        _check_block_scales("scales", scales, codes)
+        for name, t in (("x", x), ("codes", codes)):
+            if not t.is_cuda:
+                raise ValueError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
+            if t.stride(-1) != 1:
+                raise ValueError(f"the last axis of {name} must be contiguous")
+        if x.device != codes.device:
+            raise ValueError(f"codes is on {codes.device}, x on {x.device}")
+        if x.numel() == 0:
+            return
+        n, (xs, cs, ss) = _row_axes(x, codes, scales)
+        if max(n) > 2 ** 31 - 1:
+            raise ValueError("too many rows")
+        a = FdkMxfp4Args()
+        a.struct_size = C.sizeof(FdkMxfp4Args)
+        a.n, a.x_stride, a.codes_stride, a.scales_stride = (C.c_int32 * 3)(*n), (C.c_int64 * 3)(*xs), (C.c_int64 * 3)(*cs), (C.c_int64 * 3)(*ss)
+        a.num_values, a.x_dtype = d, _fdk_dtype(x.dtype, "x")
     a.x, a.codes, a.scales = x.data_ptr(), codes.data_ptr(), scales.data_ptr()
-    if max(n) > 2 ** 31 - 1:
-        raise ValueError("too many rows")
-    a.n, a.x_stride, a.codes_stride, a.scales_stride = (C.c_int32 * 3)(*n), (C.c_int64 * 3)(*xs), (C.c_int64 * 3)(*cs), (C.c_int64 * 3)(*ss)
-    a.num_values, a.x_dtype = d, _fdk_dtype(x.dtype, "x")
     _launch_on(x.device, stream, fn, a)
+    if hit is None:
+        if len(_MXFP4_TEMPLATES) >= 256:
+            _MXFP4_TEMPLATES.clear()
+        _MXFP4_TEMPLATES[key] = bytes(a)
 
 
 def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,
