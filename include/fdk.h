@@ -211,7 +211,7 @@ typedef struct fdk_decode_args {
     int32_t reserved3;
 
     /* (revision 3) kv_dtype FDK_MXFP4: the scale bytes of the caches, [num_pages, P, Hkv, D/32], with byte strides of the
-     * page, token and head axes (any alignment).  k_scale / v_scale are not read.  Built for head_dim 64, 128 and 256 with
+     * page, token and head axes; rows aligned to 4 bytes (head_dim 64: 2).  k_scale / v_scale are not read.  Built for head_dim 64, 128 and 256 with
      * v_head_dim = head_dim on the matrix-core path; no single-launch form; with counters, too, a forced split count runs as
      * one workgroup per piece.  A value takes part as code * 2^(byte - 127) converted to q's dtype, exact within its range */
     const uint8_t* k_block_scale;

@@ -104,6 +104,19 @@ def test_lengths_pages_head_dims(cuda_device, dtype, d, page):
     _run(LENS, 8, 2, d, page, dtype, 10 * d + page, cuda_device=cuda_device)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hkv", [2, 4, 8, 12])
+@pytest.mark.parametrize("page", [16, 64])
+def test_pairs_of_neighbouring_heads(cuda_device, dtype, d, hkv, page):
+    """Pairs of kv heads, staged through LDS (d = 128) or in registers: chunks, a single pass, equal shares; groups that leave
+    columns empty and groups of more than one tile of q heads."""
+    _run(LENS, 2 * hkv, hkv, d, page, dtype, 50 + hkv, cuda_device=cuda_device)
+    _run([100, 0, 17, 260, 129], 20 * hkv, hkv, d, page, dtype, 51 + hkv, kv_split=1, cuda_device=cuda_device)
+    _run([1500, 3, 0, 640], 3 * hkv, hkv, d, page, dtype, 52 + hkv, force_balanced=True, cuda_device=cuda_device)
+    _run([700, 2100], hkv, hkv, d, page, dtype, 53 + hkv, kv_split=5, soft_cap=20.0, cuda_device=cuda_device)
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (6, 2), (16, 1), (17, 1), (40, 1), (96, 3), (64, 8), (20, 4)])
 @pytest.mark.parametrize("layout", ["token", "head"])
 def test_head_layouts(cuda_device, hq, hkv, layout):

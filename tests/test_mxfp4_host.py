@@ -24,7 +24,7 @@ def _args(**kw):
     a.q_stride_b, a.q_stride_h = 32 * 128, 128
     a.k_stride_page, a.k_stride_tok, a.k_stride_head = 16 * 8 * 64, 8 * 64, 64
     a.v_stride_page, a.v_stride_tok, a.v_stride_head = 16 * 8 * 64, 8 * 64, 64
-    a.k_block_scale, a.v_block_scale = 0x80001, 0x90003
+    a.k_block_scale, a.v_block_scale = 0x80004, 0x9000C
     a.kbs_stride_page, a.kbs_stride_tok, a.kbs_stride_head = 16 * 8 * 4, 8 * 4, 4
     a.vbs_stride_page, a.vbs_stride_tok, a.vbs_stride_head = 16 * 8 * 4, 8 * 4, 4
     a.table_stride_b = 256
@@ -59,6 +59,7 @@ def test_valid_calls_pass_a_dry_run():
     ("q_dtype", _lib.FDK_MXFP4, _lib.FDK_EUNSUPPORTED), ("out_dtype", _lib.FDK_MXFP4, _lib.FDK_EUNSUPPORTED),
     ("k_stride_head", 32, _lib.FDK_ESHAPE), ("k_stride_tok", 8 * 64 + 8, _lib.FDK_EALIGN),
     ("kbs_stride_head", 3, _lib.FDK_ESHAPE), ("vbs_stride_tok", -1, _lib.FDK_ESHAPE),
+    ("k_block_scale", 0x80002, _lib.FDK_EALIGN), ("v_block_scale", 0x90001, _lib.FDK_EALIGN), ("kbs_stride_tok", 34, _lib.FDK_EALIGN),
     ("kbs_stride_page", 1 << 32, _lib.FDK_ESHAPE), ("vbs_stride_tok", 1 << 62, _lib.FDK_ESHAPE),
 ])
 def test_refusals(field, value, code):
@@ -75,8 +76,8 @@ def test_a_caller_of_the_previous_revision_is_asked_for_scales():
 
 
 def test_plans():
-    """Two kv heads per workgroup where their rows share lines (heads side by side, rows below 128 bytes), unless only one each
-    fills the compute units; short batches are cut into chunks, long ragged ones into equal shares."""
+    """Two kv heads per workgroup where their rows share lines (heads side by side, rows below 128 bytes), unless the call is short
+    and only one each fills the compute units; short batches are cut into chunks, long ragged ones into equal shares."""
     plan = FdkPlan()
     lib = _lib.load()
 
@@ -84,10 +85,17 @@ def test_plans():
         assert lib.fdk_plan(C.byref(_args(**kw)), 0, C.byref(plan)) == 0
         assert plan.algo == _lib.FDK_ALGO_MFMA and (not plan.balanced or plan.workgroups % (8 // plan.kv_heads_per_wg) == 0)
         return plan
-    assert (of().num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 1, 0)
+    short = dict(max_pages=64, table_stride_b=64, max_kv_len=1024, min_kv_len=1024)
+    assert (of(**short).num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 1, 0)
+    long = dict(max_pages=512, table_stride_b=512, max_kv_len=8192, min_kv_len=8192)
+    assert (of(**long).num_splits, plan.kv_heads_per_wg, plan.balanced) == (2, 2, 0)
     assert (of(batch=64).num_splits, plan.kv_heads_per_wg, plan.balanced) == (1, 2, 0)
+    assert of(batch=48, **short).kv_heads_per_wg == 2                  # (384 single heads would fill 256 compute units unevenly)
+    assert of(page_size=1, max_pages=4096, table_stride_b=4096, batch=64).kv_heads_per_wg == 2
+    assert of(batch=64, num_kv_heads=3, num_q_heads=6).kv_heads_per_wg == 1
     by_head = dict(k_stride_head=16 * 64, k_stride_tok=64, v_stride_head=16 * 64, v_stride_tok=64)
     assert of(batch=64, **by_head).kv_heads_per_wg == 1
+    assert (of(**by_head).num_splits, plan.kv_heads_per_wg) == (1, 1)
     wide = dict(head_dim=256, k_stride_head=128, v_stride_head=128, k_stride_tok=1024, v_stride_tok=1024)
     assert of(batch=64, **wide).kv_heads_per_wg == 1
     assert of(batch=64, num_kv_heads=1, num_q_heads=8).kv_heads_per_wg == 1

@@ -43,6 +43,7 @@ SOURCES = [
     "fdk_attn_weights.hip", "fdk_kv_evict.hip",
     # MXFP4 caches; appends with explicit positions
     "fdk_kv_append_axes.hip", "fdk_mxfp4.hip", "fdk_splitkv_mx4_d64.hip", "fdk_splitkv_mx4_d128.hip", "fdk_splitkv_mx4_d256.hip",
+    "fdk_splitkv_mx4_staged.hip",
 ]
 
 # the translation units that contain the matrix-core split kernel: the only ones the timeline build compiles anew

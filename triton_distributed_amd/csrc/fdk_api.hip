@@ -164,11 +164,14 @@ inline bool plain_dims(int dk, int dv) { return dk == dv && (dk == 64 || dk == 1
 inline bool two_segment_dims(int dk, int dv) { return (dk == 192 && (dv == 192 || dv == 128)) || (dk == 576 && dv == 512); }
 
 // byte strides of an MXFP4 cache's scales (page, token, head)
-int check_scale_strides(int64_t sp, int64_t st, int64_t sh, int head_dim, int num_kv_heads, int page_size) {
+int check_scale_strides(const void* scales, int64_t sp, int64_t st, int64_t sh, int head_dim, int num_kv_heads, int page_size) {
     if (sp < 0 || st < 0 || sh < 0) return fail(FDK_ESHAPE, "negative block scale stride");
     if (num_kv_heads > 1 && sh < head_dim / fdk::kMxBlock) return fail(FDK_ESHAPE, "block scale head stride < head_dim / 32");
     if (sp >= ((int64_t)1 << 32) || st >= ((int64_t)1 << 28) || page_size * st >= ((int64_t)1 << 32))
         return fail(FDK_ESHAPE, "block scale strides too large: a page must span less than 4 GiB");
+    // (scales: null where the alignment does not matter)
+    const int64_t odd = !scales ? 0 : (int64_t)reinterpret_cast<uintptr_t>(scales) | sp | st | (num_kv_heads > 1 ? sh : 0);
+    if (odd & (head_dim >= 128 ? 3 : 1)) return fail(FDK_EALIGN, "block scales of a row must be aligned to %d bytes", head_dim >= 128 ? 4 : 2);
     return FDK_OK;
 }
 
@@ -266,7 +269,7 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
         const int64_t bs[2][3] = {{a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head},
                                   {a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head}};
         for (const auto& b : bs)
-            if (int rc = check_scale_strides(b[0], b[1], b[2], a->head_dim, a->num_kv_heads, a->page_size)) return rc;
+            if (int rc = check_scale_strides(&b == bs ? a->k_block_scale : a->v_block_scale, b[0], b[1], b[2], a->head_dim, a->num_kv_heads, a->page_size)) return rc;
     }
     if (a->table_stride_b < a->max_pages)
         return fail(FDK_ESHAPE, "table_stride_b %lld < max_pages %d", (long long)a->table_stride_b, a->max_pages);
@@ -287,12 +290,16 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
 }
 
 // kv heads per workgroup of the MXFP4 kernels: two where rows of neighbouring heads are parts of the same 128-byte lines, so that
-// one compute unit reads whole lines - unless only single heads give every compute unit a workgroup, and with it a single pass:
-// the combine launch then costs what the whole lines save (batch 32 x 8 kv heads x 4096 tokens: 36 us either way).
-int mx_kv_heads_per_wg(const fdk_decode_args* a, int64_t head_units, int num_cus) {
+// one compute unit reads whole lines - unless only single heads give every compute unit (evenly) a workgroup, and with it a single
+// pass, and the call is short: the combine launch then costs more than the whole lines save (batch 32 x 8 kv heads, rows of 64 bytes,
+// single heads against pairs: 10 / 17 us at 1024 tokens, 20 / 25 at 2048, 37 / 37 at 4096, 70 / 60 at 8192; rows of 32 bytes: 13 / 15
+// at 2048, 27 / 24 at 4096; batch 48, an uneven fill, 64-byte rows: 67 / 49 at 4096).
+int mx_kv_heads_per_wg(const fdk_decode_args* a, int64_t head_units, int num_cus, double stream_us) {
     const bool neighbours = a->k_stride_head == a->head_dim / 2 && a->v_stride_head == a->head_dim / 2;
     if (!neighbours || a->head_dim > 128 || a->num_kv_heads % 2) return 1;
-    return head_units >= num_cus && head_units / 2 < num_cus ? 1 : 2;
+    const bool only_single = head_units >= num_cus && head_units / 2 < num_cus;
+    const bool even = head_units * 10 >= cdiv64(head_units, num_cus) * num_cus * 9;
+    return only_single && even && stream_us < a->head_dim / 6 ? 1 : 2;
 }
 
 int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
@@ -321,9 +328,13 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
     int kv_heads_per_wg = 1;
     int units_per_seq;
     const int tile_heads = algo == FDK_ALGO_MFMA ? fdk::mfma_heads_per_wg(group, a->head_dim + v_dim(a), a->kv_dtype) : 16;   // q heads of a kv head per workgroup
+    // what streaming the batch's cache takes (the shared-tile kernels are bound by the 16-bit tile they stage, not by
+    // the bytes they read: a one-byte cache takes them as long as a 16-bit one, and is planned like one)
+    const double stream_us = (double)batch * (double)max_len * a->num_kv_heads *
+                             kv_bytes(tile_heads > 16 ? FDK_BF16 : a->kv_dtype, (double)(a->head_dim + v_dim(a))) / kStreamBytesPerUs;
     if (algo == FDK_ALGO_MFMA) {
         kv_heads_per_wg = a->kv_dtype == FDK_MXFP4
-                              ? mx_kv_heads_per_wg(a, (int64_t)batch * a->num_kv_heads * ((group + 15) / 16), num_cus)
+                              ? mx_kv_heads_per_wg(a, (int64_t)batch * a->num_kv_heads * ((group + 15) / 16), num_cus, stream_us)
                               : fdk::mfma_kv_heads_per_wg(batch, a->num_kv_heads, group, num_cus, a->head_dim + v_dim(a), a->kv_dtype);
         units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
     } else {
@@ -344,10 +355,6 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
     //    pass runs at (fill + 1) / 2 of the even rate, fill = units / (rounds x compute units): 131 / 139 /
     //    159 us against 103 / 124 / 155 us of streaming time.
     const bool alike = a->min_kv_len > 0 && (int64_t)a->min_kv_len * 32 >= max_len * 31;
-    // what streaming the batch's cache takes (the shared-tile kernels are bound by the 16-bit tile they stage, not by
-    // the bytes they read: a one-byte cache takes them as long as a 16-bit one, and is planned like one)
-    const double stream_us = (double)batch * (double)max_len * a->num_kv_heads *
-                             kv_bytes(tile_heads > 16 ? FDK_BF16 : a->kv_dtype, (double)(a->head_dim + v_dim(a))) / kStreamBytesPerUs;
     bool rebalance = false;
     // (measurement aid: equal shares wherever they can run, to time them against the plan chosen here)
     const bool force_balanced = a->measure && a->measure->force_balanced && algo == FDK_ALGO_MFMA && a->num_splits <= 0 &&
@@ -365,7 +372,7 @@ int make_plan(const fdk_decode_args* a, int num_cus, fdk_plan_t* plan) {
         if (rebalance) {
             kv_heads_per_wg = a->num_kv_heads % 2 ? 1 : 2;
             if (tile_heads > 16) kv_heads_per_wg = 1;
-            if (a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = mx_kv_heads_per_wg(a, 0, num_cus);
+            if (a->kv_dtype == FDK_MXFP4) kv_heads_per_wg = mx_kv_heads_per_wg(a, 0, num_cus, stream_us);
             units_per_seq = fdk::mfma_units_per_seq(a->num_kv_heads, group, kv_heads_per_wg, tile_heads);
         }
     }
@@ -938,8 +945,8 @@ static int kv_append(const fdk_kv_append_args* caller_args, const fdk_kv_append_
     if (mx) {
         if (!x->k_block_scale || !x->v_block_scale)
             return fail(FDK_ENULL, "k_block_scale / v_block_scale are required for an mxfp4 cache");
-        int rc = check_scale_strides(x->kbs_stride_page, x->kbs_stride_tok, x->kbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
-        if (!rc) rc = check_scale_strides(x->vbs_stride_page, x->vbs_stride_tok, x->vbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
+        int rc = check_scale_strides(nullptr, x->kbs_stride_page, x->kbs_stride_tok, x->kbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
+        if (!rc) rc = check_scale_strides(nullptr, x->vbs_stride_page, x->vbs_stride_tok, x->vbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
         if (rc) return rc;
         int64_t odd = 0;
         for (int i = 0; i < 6; ++i) odd |= st[i];
@@ -1065,7 +1072,7 @@ int fdk_accumulate_weights(const fdk_attn_weights_args* caller_args, void* hip_s
         return fail(FDK_ESHAPE, "weights rows overlap");
     if (mx) {
         if (!a->k_block_scale) return fail(FDK_ENULL, "k_block_scale is required for an mxfp4 cache");
-        if (int rc = check_scale_strides(a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head, d, a->num_kv_heads, a->page_size)) return rc;
+        if (int rc = check_scale_strides(nullptr, a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head, d, a->num_kv_heads, a->page_size)) return rc;
     }
     const bool dry = (a->flags & FDK_FLAG_DRY_RUN) != 0;
     const int cus = dry ? kDryRunCus : query_cus();
@@ -1129,8 +1136,8 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     if (mx) {
         if (!a->k_block_scale || !a->v_block_scale)
             return fail(FDK_ENULL, "k_block_scale / v_block_scale are required for an mxfp4 cache");
-        int rc = check_scale_strides(a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
-        if (!rc) rc = check_scale_strides(a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head, dv, a->num_kv_heads, a->page_size);
+        int rc = check_scale_strides(nullptr, a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head, a->head_dim, a->num_kv_heads, a->page_size);
+        if (!rc) rc = check_scale_strides(nullptr, a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head, dv, a->num_kv_heads, a->page_size);
         if (rc) return rc;
     }
     if (!a->weights || !a->weights_out || !a->kept || !a->kv_lens_out)

@@ -8,8 +8,11 @@ FDK_DECLARE_MX4(64)
 FDK_DECLARE_MX4(128)
 FDK_DECLARE_MX4(256)
 #undef FDK_DECLARE_MX4
+int launch_splitkv_mx4_staged(const SplitParams& p, const Mx4Scales& x, int q_dtype, hipStream_t stream);
 
 int launch_splitkv_mx4(const SplitParams& p, const Mx4Scales& x, int q_dtype, hipStream_t stream) {
+    // pairs of 64-byte rows (one line), pages of 16 << n tokens: through LDS
+    if (p.head_dim == 128 && p.hg_per_wg == 2 && p.page_shift >= 4) return launch_splitkv_mx4_staged(p, x, q_dtype, stream);
     switch (p.head_dim) {
         case 64: return launch_splitkv_mx4_d64(p, x, q_dtype, stream);
         case 128: return launch_splitkv_mx4_d128(p, x, q_dtype, stream);

@@ -42,15 +42,210 @@ struct Mx4Tile {                           // one step in registers, as loaded
     uint32_t vs[2][VS];
 };
 
+// What a wavefront does with a step of 32 tokens of one kv head, and how the wavefronts of a head are merged.  Lane (c, a):
+// q head c of the tile, tokens 16 hf + a + 4 i of the step.
+template <int QDT, int D>
+struct Mx4Math {
+    using P2 = Pack2<QDT>;
+    using T = Mx4Tile<D>;
+    static constexpr int DB = D / 16;          // column blocks of O^T, values of a V row per lane
+    static constexpr int KSTEPS = D / 32;      // MFMA steps of a K row
+
+    static __device__ __forceinline__ f32x4_t mma(uint4 a, uint4 b, f32x4_t c) { return Mma<QDT>::qk(a, b, c); }     // 16 x 16 x 32
+
+    // the scales of the lane group's four tokens, from the four lanes (two pairs of lanes) that loaded them
+    static __device__ __forceinline__ void v_scales(const uint32_t (&in)[T::VS], float* sc) {
+        if constexpr (T::VS == 1) {
+            const float x0 = mx_scale(in[0]);
+            sc[0] = dpp_mov<0x00>(x0);                         // quad_perm [0,0,0,0] ...
+            sc[1] = dpp_mov<0x55>(x0);
+            sc[2] = dpp_mov<0xAA>(x0);
+            sc[3] = dpp_mov<0xFF>(x0);
+        } else {
+            const float x0 = mx_scale(in[0]), x1 = mx_scale(in[1]);
+            sc[0] = dpp_mov<0xA0>(x0);                         // quad_perm [0,0,2,2]
+            sc[1] = dpp_mov<0xF5>(x0);                         // quad_perm [1,1,3,3]
+            sc[2] = dpp_mov<0xA0>(x1);
+            sc[3] = dpp_mov<0xF5>(x1);
+        }
+    }
+
+    // ---- S^T[token][head] = K Q^T, two tiles of 16 tokens: sv[4 hf + i] is token 16 hf + a + 4 i ----
+    static __device__ __forceinline__ void scores(const T& r, const uint4 (&q)[KSTEPS], float (&sv)[8]) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks) {
+                const float sc = mx_scale(r.ks[hf][T::KS == 2 ? ks / 4 : 0]);
+                const uint32_t w = r.k[hf][ks];
+                s = mma(make_uint4(mx_unpack2<QDT, 0>(w, sc), mx_unpack2<QDT, 1>(w, sc), mx_unpack2<QDT, 2>(w, sc),
+                                   mx_unpack2<QDT, 3>(w, sc)), q[ks], s);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sv[4 * hf + i] = s[i];
+        }
+    }
+
+    // ---- online softmax for head c over this lane group's eight tokens; the probabilities as operand B of P V.  MASKED: only
+    // the first `left` tokens of the step (at least one) take part ----
+    template <typename MaskedTag>
+    static __device__ __forceinline__ uint4 softmax(float (&sv)[8], float& m_run, float& l_run, f32x4_t (&acc)[DB], const SplitParams& p,
+                                                    float inv_cap, int a, int left, MaskedTag) {
+        if (p.soft_cap > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sv[i] = soft_cap_fn(sv[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sv[i] *= p.scale_log2;
+        }
+        if (MaskedTag::value) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (16 * (i >> 2) + a + 4 * (i & 3) >= left) sv[i] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+        mx = max_across_rows(mx);
+        // The running maximum moves only when a step exceeds it by more than 2^8: probabilities of up to 256 are as exact
+        // in 16 bits and in the fp32 sums as those below 1, and the accumulators are rescaled a few times per piece.
+        // (fp16: the reference stays 2^7 below the maximum, so that probabilities down to 2^-21 of the largest are normal fp16
+        // values; the largest is then at most 2^15.)
+        constexpr float kBelow = QDT == FDK_FP16 ? 7.0f : 0.0f;
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + (8.0f + kBelow)) != 0) {
+            const float m_new = fmaxf(m_run, mx - kBelow);
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+            m_run = m_new;
+        }
+        float pr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(sv[i] - m_run);
+        l_run += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+        // probabilities rounded to the q dtype, as the 16-bit kernels do; the sum above is of the unrounded ones
+        return make_uint4(P2::pack(pr[0], pr[1]), P2::pack(pr[2], pr[3]), P2::pack(pr[4], pr[5]), P2::pack(pr[6], pr[7]));
+    }
+
+    // ---- O^T[value][head] += V^T P^T ----
+    static __device__ __forceinline__ void values(const T& r, const uint4 pv, f32x4_t (&o)[DB]) {
+        float sc[8];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) v_scales(r.vs[hf], sc + 4 * hf);
+        auto pair = [&](auto byte_tag, int w, int db) {        // column blocks db, db + 1: byte `byte_tag` of the V words
+            constexpr int BY = decltype(byte_tag)::value;
+            uint32_t u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] = mx_unpack2<QDT, BY>(r.v[j][w], sc[j]);
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x05040100u);
+                hi[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
+            }
+            o[db] = mma(make_uint4(lo[0], lo[1], lo[2], lo[3]), pv, o[db]);
+            o[db + 1] = mma(make_uint4(hi[0], hi[1], hi[2], hi[3]), pv, o[db + 1]);
+        };
+#pragma unroll
+        for (int w = 0; w < T::VW; ++w) {
+            pair(IntTag<0>(), w, 8 * w);
+            pair(IntTag<1>(), w, 8 * w + 2);
+            if constexpr (D >= 128) {
+                pair(IntTag<2>(), w, 8 * w + 4);
+                pair(IntTag<3>(), w, 8 * w + 6);
+            }
+        }
+    }
+
+    // A wavefront's part of the merge: block e = i (DB / 4) + q of its D * 64 bytes holds, per lane, the values
+    // DB (4 a + i) + 4 q .. + 3 of head c - every LDS instruction touches one contiguous kilobyte, and a merging lane stores
+    // four consecutive values -; m and l: [16]
+    static __device__ __forceinline__ void leave_part(const f32x4_t (&acc)[DB], float m_run, float l_run, char* part, float* m, float* l,
+                                                      bool live, int lane) {
+        l_run += __shfl_xor(l_run, 16, 64);
+        l_run += __shfl_xor(l_run, 32, 64);
+        if (!live) return;
+        float4* o = reinterpret_cast<float4*>(part);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int q = 0; q < DB / 4; ++q)
+                o[(i * (DB / 4) + q) * 64 + lane] = make_float4(acc[4 * q][i], acc[4 * q + 1][i], acc[4 * q + 2][i], acc[4 * q + 3][i]);
+        if (lane < 16) {
+            m[lane] = m_run;
+            l[lane] = l_run;
+        }
+    }
+    // TI parts of one kv head, `stride` bytes apart (m, l: ml_stride values apart), by the TI wavefronts that left them: this one
+    // takes the blocks e = first, first + TI ...  Row: q head hq of the result, or partial row prow.
+    template <int TI>
+    static __device__ __forceinline__ void merge_parts(const SplitParams& p, const char* parts, int stride, const float* m, const float* l,
+                                                       int ml_stride, int first, int b, int hq, int64_t prow, int lane) {
+        const int a = lane >> 4, c = lane & 15;
+        float mw[TI], lw[TI];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < TI; ++t) {
+            mw[t] = m[t * ml_stride + c];
+            lw[t] = l[t * ml_stride + c];
+            mx = fmaxf(mx, mw[t]);
+        }
+        float sc[TI], sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < TI; ++t) {
+            sc[t] = fast_exp2(mw[t] - mx);               // mx is finite: the piece holds a token
+            sum += lw[t] * sc[t];
+        }
+        const float norm = fast_rcp(sum);
+        const float lse_nat = (mx + fast_log2(sum)) * kLn2;
+#pragma unroll
+        for (int t = 0; t < TI; ++t) sc[t] *= norm;
+        for (int e = first; e < DB; e += TI) {
+            float4 xw[TI];
+#pragma unroll
+            for (int t = 0; t < TI; ++t) xw[t] = reinterpret_cast<const float4*>(parts + t * stride)[e * 64 + lane];
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int t = 0; t < TI; ++t) {
+                o.x += xw[t].x * sc[t];
+                o.y += xw[t].y * sc[t];
+                o.z += xw[t].z * sc[t];
+                o.w += xw[t].w * sc[t];
+            }
+            const int d0 = DB * (4 * a + e / (DB / 4)) + 4 * (e % (DB / 4));
+            if (p.direct) store_out4(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + d0, o, p.out_dtype);
+            else *reinterpret_cast<float4*>(p.part_o + prow * D + d0) = o;
+        }
+        if (first == 0 && a == 0) {
+            if (p.direct) {
+                if (p.lse) p.lse[(int64_t)b * p.lse_sb + hq] = lse_nat;
+                if (p.pack_lse) store_out(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + D, lse_nat, p.out_dtype);
+            } else {
+                p.part_lse[prow] = lse_nat;
+            }
+        }
+    }
+    // out = 0, lse = -inf for the q heads [head0, head0 + heads_here) of an empty sequence; one wavefront
+    static __device__ __forceinline__ void write_empty_rows(const SplitParams& p, int b, int head0, int heads_here, int lane) {
+        for (int idx = lane; idx < heads_here * D; idx += 64) {
+            const int g = idx / D, d = idx % D;
+            const int64_t ob = (int64_t)b * p.out_sb + (int64_t)(head0 + g) * p.out_sh;
+            store_out(p.out, ob + d, 0.f, p.out_dtype);
+            if (d == 0) {
+                if (p.lse) p.lse[(int64_t)b * p.lse_sb + head0 + g] = -INFINITY;
+                if (p.pack_lse) store_out(p.out, ob + D, -INFINITY, p.out_dtype);
+            }
+        }
+    }
+};
+
 // NH: kv heads of a workgroup (neighbours in memory: their rows share lines).  STREAM: every line is one workgroup's alone, and
 // is loaded with the non-temporal hint; otherwise plain loads leave the lines in the L2 for the next reader.
 template <int QDT, int PM, int D, int MODE, int NH, bool STREAM>
 __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, const Mx4Scales x) {
     static_assert(PM == PM_TILE || PM == PM_ROW, "page numbers per tile of 16 tokens, or per row");
     static_assert(!STREAM || NH == 1, "two buffers of one kv head's rows");
-    using P2 = Pack2<QDT>;
     using T = Mx4Tile<D>;
-    constexpr int DV = D;
     constexpr int DB = D / 16;                 // column blocks of O^T, values of a V row per lane
     constexpr int KSTEPS = D / 32;             // MFMA steps of a K row
     constexpr int kTileHeads = 16;
@@ -71,17 +266,8 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     float* sm_l = sm_m + nw * NH * 16;
     int* const s_next = reinterpret_cast<int*>(sm_l + nw * NH * 16);
 
-    // out = 0, lse = -inf for the q heads [head0, head0 + heads_here) of an empty sequence; one wavefront
     auto write_empty_rows = [&](const int b, const int head0, const int heads_here) {
-        for (int idx = lane; idx < heads_here * DV; idx += 64) {
-            const int g = idx / DV, d = idx % DV;
-            const int64_t ob = (int64_t)b * p.out_sb + (int64_t)(head0 + g) * p.out_sh;
-            store_out(p.out, ob + d, 0.f, p.out_dtype);
-            if (d == 0) {
-                if (p.lse) p.lse[(int64_t)b * p.lse_sb + head0 + g] = -INFINITY;
-                if (p.pack_lse) store_out(p.out, ob + DV, -INFINITY, p.out_dtype);
-            }
-        }
+        Mx4Math<QDT, D>::write_empty_rows(p, b, head0, heads_here, lane);
     };
 
     // One piece: tokens [c_start, min(c_limit, kv_len)) of sequence b for kv heads NH hgb .. NH hgb + NH - 1 and q-head tile ht;
@@ -129,8 +315,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
         return;
     }
     const int c_end = min(c_limit, kv_len);
-    const bool softcap = p.soft_cap > 0.f;
-    const float inv_cap = softcap ? 1.0f / p.soft_cap : 0.f;
+    const float inv_cap = p.soft_cap > 0.f ? 1.0f / p.soft_cap : 0.f;
 
     const char* kplane = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh;
     const char* vplane = reinterpret_cast<const char*>(p.v) + (int64_t)kvh * p.v_sh;
@@ -260,101 +445,9 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
         for (int db = 0; db < DB; ++db) acc[h][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // the scales of the lane group's four tokens, from the four lanes (two pairs of lanes) that loaded them
-    auto v_scales = [&](const uint32_t (&in)[T::VS], float* sc) {
-        if constexpr (T::VS == 1) {
-            const float x0 = mx_scale(in[0]);
-            sc[0] = dpp_mov<0x00>(x0);                         // quad_perm [0,0,0,0] ...
-            sc[1] = dpp_mov<0x55>(x0);
-            sc[2] = dpp_mov<0xAA>(x0);
-            sc[3] = dpp_mov<0xFF>(x0);
-        } else {
-            const float x0 = mx_scale(in[0]), x1 = mx_scale(in[1]);
-            sc[0] = dpp_mov<0xA0>(x0);                         // quad_perm [0,0,2,2]
-            sc[1] = dpp_mov<0xF5>(x0);                         // quad_perm [1,1,3,3]
-            sc[2] = dpp_mov<0xA0>(x1);
-            sc[3] = dpp_mov<0xF5>(x1);
-        }
-    };
-    auto mma = [&](uint4 av, uint4 bv, f32x4_t cv) { return Mma<QDT>::qk(av, bv, cv); };     // 16 x 16 x 32
-    // ---- S^T[token][head] = K Q^T, two tiles of 16 tokens: sv[4 hf + i] is token 16 hf + a + 4 i ----
-    auto scores = [&](const T& r, const uint4 (&q)[KSTEPS], float (&sv)[8]) {
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KSTEPS; ++ks) {
-                const float sc = mx_scale(r.ks[hf][T::KS == 2 ? ks / 4 : 0]);
-                const uint32_t w = r.k[hf][ks];
-                s = mma(make_uint4(mx_unpack2<QDT, 0>(w, sc), mx_unpack2<QDT, 1>(w, sc), mx_unpack2<QDT, 2>(w, sc),
-                                   mx_unpack2<QDT, 3>(w, sc)), q[ks], s);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sv[4 * hf + i] = s[i];
-        }
-    };
-    // ---- online softmax for head c over this lane group's eight tokens; the probabilities as operand B of P V ----
+    using Math = Mx4Math<QDT, D>;
     auto softmax = [&](int t, float (&sv)[8], int h, auto masked_tag) {
-        if (softcap) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sv[i] = soft_cap_fn(sv[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sv[i] *= p.scale_log2;
-        }
-        if (decltype(masked_tag)::value) {
-            const int tok0 = c_start + t * kStep;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (tok0 + 16 * (i >> 2) + a + 4 * (i & 3) >= c_end) sv[i] = -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-        mx = max_across_rows(mx);
-        // The running maximum moves only when a step exceeds it by more than 2^8: probabilities of up to 256 are as exact
-        // in 16 bits and in the fp32 sums as those below 1, and the accumulators are rescaled a few times per piece.
-        if (__builtin_amdgcn_ballot_w64(mx > m_run[h] + 8.0f) != 0) {
-            const float m_new = fmaxf(m_run[h], mx);
-            const float alpha = fast_exp2(m_run[h] - m_new);
-            l_run[h] *= alpha;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) acc[h][db] *= alpha;
-            m_run[h] = m_new;
-        }
-        float pr[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(sv[i] - m_run[h]);
-        l_run[h] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-        // probabilities rounded to the q dtype, as the 16-bit kernels do; the sum above is of the unrounded ones
-        return make_uint4(P2::pack(pr[0], pr[1]), P2::pack(pr[2], pr[3]), P2::pack(pr[4], pr[5]), P2::pack(pr[6], pr[7]));
-    };
-    // ---- O^T[value][head] += V^T P^T ----
-    auto values = [&](const T& r, const uint4 pv, f32x4_t (&o)[DB]) {
-        float sc[8];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) v_scales(r.vs[hf], sc + 4 * hf);
-        auto pair = [&](auto byte_tag, int w, int db) {        // column blocks db, db + 1: byte `byte_tag` of the V words
-            constexpr int BY = decltype(byte_tag)::value;
-            uint32_t u[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) u[j] = mx_unpack2<QDT, BY>(r.v[j][w], sc[j]);
-            uint32_t lo[4], hi[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                lo[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x05040100u);
-                hi[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
-            }
-            o[db] = mma(make_uint4(lo[0], lo[1], lo[2], lo[3]), pv, o[db]);
-            o[db + 1] = mma(make_uint4(hi[0], hi[1], hi[2], hi[3]), pv, o[db + 1]);
-        };
-#pragma unroll
-        for (int w = 0; w < T::VW; ++w) {
-            pair(IntTag<0>(), w, 8 * w);
-            pair(IntTag<1>(), w, 8 * w + 2);
-            if constexpr (D >= 128) {
-                pair(IntTag<2>(), w, 8 * w + 4);
-                pair(IntTag<3>(), w, 8 * w + 6);
-            }
-        }
+        return Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, c_end - (c_start + t * kStep), masked_tag);
     };
 
     // ---- pipeline ----
@@ -375,8 +468,8 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
             T r2[NH];
             auto work = [&](int tw, const T (&rw)[NH]) {
                 float sv[8];
-                scores(rw[0], qb[0], sv);
-                values(rw[0], softmax(tw, sv, 0, BoolTag<false>()), acc[0]);
+                Math::scores(rw[0], qb[0], sv);
+                Math::values(rw[0], softmax(tw, sv, 0, BoolTag<false>()), acc[0]);
             };
             while (t + 2 * st < n_full) {
                 fetch_pages(t + 2 * st, p.max_tokens - 1, pa);
@@ -405,13 +498,13 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
                 if (kIdsFirst) fetch_pages(tn + st, p.max_tokens - 1, pa);
                 float sv[NH][8];
 #pragma unroll
-                for (int h = 0; h < NH; ++h) scores(r[h], qb[h], sv[h]);
+                for (int h = 0; h < NH; ++h) Math::scores(r[h], qb[h], sv[h]);
                 if (more) issue_k(tn, pb, r, BoolTag<false>());
                 uint4 pv[NH];
 #pragma unroll
                 for (int h = 0; h < NH; ++h) pv[h] = softmax(t, sv[h], h, BoolTag<false>());
 #pragma unroll
-                for (int h = 0; h < NH; ++h) values(r[h], pv[h], acc[h]);
+                for (int h = 0; h < NH; ++h) Math::values(r[h], pv[h], acc[h]);
                 if (more) issue_v(tn, pb, r, BoolTag<false>());
                 if (!kIdsFirst) fetch_pages(tn + st, p.max_tokens - 1, pa);
                 pb = pa;
@@ -425,85 +518,24 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
                 float sv[8];
-                scores(r[h], qb[h], sv);
-                values(r[h], softmax(n_full, sv, h, BoolTag<true>()), acc[h]);
+                Math::scores(r[h], qb[h], sv);
+                Math::values(r[h], softmax(n_full, sv, h, BoolTag<true>()), acc[h]);
             }
         }
     }
 
-    // ---- merge: lane groups (sum of l), then the wavefronts through LDS ----
-    // Block e = i (DB / 4) + q of a wavefront's scratch holds, per lane, its values DB (4 a + i) + 4 q .. + 3 of head c: every
-    // LDS instruction touches one contiguous kilobyte, and a merging lane stores four consecutive values.
+    // ---- merge of the wavefronts through LDS ----
     const bool live = c < heads_here;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-        l_run[h] += __shfl_xor(l_run[h], 16, 64);
-        l_run[h] += __shfl_xor(l_run[h], 32, 64);
-        float4* my_o = reinterpret_cast<float4*>(lds + (wave * NH + h) * kScratch);
-        if (live) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int q = 0; q < DB / 4; ++q)
-                    my_o[(i * (DB / 4) + q) * 64 + lane] =
-                        make_float4(acc[h][4 * q][i], acc[h][4 * q + 1][i], acc[h][4 * q + 2][i], acc[h][4 * q + 3][i]);
-            if (a == 0) {
-                sm_m[(wave * NH + h) * 16 + c] = m_run[h];
-                sm_l[(wave * NH + h) * 16 + c] = l_run[h];
-            }
-        }
-    }
+    for (int h = 0; h < NH; ++h)
+        Math::leave_part(acc[h], m_run[h], l_run[h], lds + (wave * NH + h) * kScratch, sm_m + (wave * NH + h) * 16, sm_l + (wave * NH + h) * 16,
+                         live, lane);
     __syncthreads();
     if (live) {
-        auto merge = [&](auto share_tag, int h) {
-            constexpr int TI = decltype(share_tag)::value;
-            const int hq = head0 + h * p.group + c;
-            const int64_t prow = prow0 + h * kv_step + (int64_t)c * prow_step;
-            float mw[TI], lw[TI];
-            float mx = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < TI; ++t) {
-                mw[t] = sm_m[(t * NH + h) * 16 + c];
-                lw[t] = sm_l[(t * NH + h) * 16 + c];
-                mx = fmaxf(mx, mw[t]);
-            }
-            float sc[TI], l = 0.f;
-#pragma unroll
-            for (int t = 0; t < TI; ++t) {
-                sc[t] = fast_exp2(mw[t] - mx);               // mx is finite: the piece holds a token
-                l += lw[t] * sc[t];
-            }
-            const float norm = fast_rcp(l);
-            const float lse_nat = (mx + fast_log2(l)) * kLn2;
-#pragma unroll
-            for (int t = 0; t < TI; ++t) sc[t] *= norm;
-            for (int e = wave; e < DB; e += TI) {
-                float4 xw[TI];
-#pragma unroll
-                for (int t = 0; t < TI; ++t) xw[t] = reinterpret_cast<const float4*>(lds + (t * NH + h) * kScratch)[e * 64 + lane];
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int t = 0; t < TI; ++t) {
-                    o.x += xw[t].x * sc[t];
-                    o.y += xw[t].y * sc[t];
-                    o.z += xw[t].z * sc[t];
-                    o.w += xw[t].w * sc[t];
-                }
-                const int d0 = DB * (4 * a + e / (DB / 4)) + 4 * (e % (DB / 4));
-                if (p.direct) store_out4(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + d0, o, p.out_dtype);
-                else *reinterpret_cast<float4*>(p.part_o + prow * DV + d0) = o;
-            }
-            if (wave == 0 && a == 0) {
-                if (p.direct) {
-                    if (p.lse) p.lse[(int64_t)b * p.lse_sb + hq] = lse_nat;
-                    if (p.pack_lse) store_out(p.out, (int64_t)b * p.out_sb + (int64_t)hq * p.out_sh + DV, lse_nat, p.out_dtype);
-                } else {
-                    p.part_lse[prow] = lse_nat;
-                }
-            }
-        };
-#pragma unroll
-        for (int h = 0; h < NH; ++h) merge(IntTag<kWaves>(), h);
+        for (int h = 0; h < NH; ++h)
+            Math::template merge_parts<kWaves>(p, lds + h * kScratch, NH * kScratch, sm_m + h * 16, sm_l + h * 16, NH * 16, wave, b,
+                                               head0 + h * p.group + c, prow0 + h * kv_step + (int64_t)c * prow_step, lane);
     }
     };   // run_piece
 #include "fdk_splitkv_mfma_work.h"
@@ -550,8 +582,15 @@ int launch_mx4(const SplitParams& p_in, const Mx4Scales& x, hipStream_t stream) 
         else FDK_MX4_LAUNCH_NH(1, false);
     } else {
         if constexpr (D <= 128) {
-            if (p.hg_per_wg != 2) return (int)hipErrorInvalidValue;
-            FDK_MX4_LAUNCH_NH(2, false);
+            // (D = 128, pages of 16 << n tokens: fdk_splitkv_mx4_staged.hip)
+            if (p.hg_per_wg != 2 || (D == 128 && tile)) return (int)hipErrorInvalidValue;
+            if constexpr (D == 64) {
+                FDK_MX4_LAUNCH_NH(2, false);
+            } else if (p.balanced) {
+                FDK_MX4_LAUNCH(PM_ROW, WM_SHARES, 2, false);
+            } else {
+                FDK_MX4_LAUNCH(PM_ROW, WM_ONE, 2, false);
+            }
         } else {
             return (int)hipErrorInvalidValue;
         }
