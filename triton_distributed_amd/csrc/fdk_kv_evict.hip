@@ -436,7 +436,7 @@ __device__ __forceinline__ void store_row(uint4* p, uint4 v) {
 }
 __device__ __forceinline__ void store_row(uint8_t* p, uint8_t v) { *p = v; }
 
-template <typename V>
+template <int THREADS, typename V>
 __device__ __forceinline__ void move_rows(const MoveParams& m, const EvictRows& r, const int lanes, const int slice, const int b,
                                           const int h, const int part) {
     constexpr int U = 8;                                   // rows of a thread that are under way together
@@ -445,7 +445,7 @@ __device__ __forceinline__ void move_rows(const MoveParams& m, const EvictRows& 
     const int4 plan = *reinterpret_cast<const int4*>(p.plan + ((int64_t)b * p.hkv + h) * 4);
     const int32_t* tbl = p.block_table + b * p.tbl_sb;
     char* base = r.pool + h * r.sh + ((int64_t)slice * lanes + threadIdx.x % lanes) * (int64_t)sizeof(V);
-    const int row = threadIdx.x / lanes, rows = 256 / lanes;
+    const int row = threadIdx.x / lanes, rows = THREADS / lanes;
     // Rows j0 + row, j0 + rows + row ... of a chunk, as far as they are below `end`.  In stages - slots, pages, rows - so that
     // each stage's loads are under way together; rows past the end repeat the last one and are not stored.
     const int chunk = rows * U;
@@ -492,14 +492,15 @@ __device__ __forceinline__ void move_rows(const MoveParams& m, const EvictRows& 
     }
 }
 
-__global__ __launch_bounds__(256) void evict_move_kernel(const MoveParams m) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void evict_move_kernel(const MoveParams m) {
     const int part = blockIdx.x % m.parts, slice = blockIdx.x / m.parts;
     const int h = blockIdx.y, b = blockIdx.z;
     if ((int)blockIdx.x >= m.row_blocks) {                // (rows of several segments) the survivors' weights
         const int64_t row = (int64_t)b * m.e.hkv + h;
         const int new_len = m.e.plan[row * 4 + 2], blocks = (int)gridDim.x - m.row_blocks;
         float* wo = m.e.weights_out + b * m.e.wo_sb + h * m.e.wo_sh;
-        for (int j = ((int)blockIdx.x - m.row_blocks) * 256 + (int)threadIdx.x; j < m.e.weights_len; j += blocks * 256)
+        for (int j = ((int)blockIdx.x - m.row_blocks) * THREADS + (int)threadIdx.x; j < m.e.weights_len; j += blocks * THREADS)
             wo[j] = j < new_len ? m.e.stash[row * m.e.keep + j] : 0.f;
         return;
     }
@@ -507,11 +508,11 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const MoveParams m) {
     if (m.parallel && blockIdx.x == 0 && h == 0 && threadIdx.x == 0)
         m.e.kv_lens_out[b] = m.e.plan[(int64_t)b * m.e.hkv * 4 + 2];
     // (written out: an index into the arrays of the argument block would put them into scratch memory)
-    if (slice < m.slices[0]) move_rows<uint4>(m, m.e.rows[0], m.lanes[0], slice, b, h, part);
-    else if (slice < m.slices[0] + m.slices[1]) move_rows<uint4>(m, m.e.rows[1], m.lanes[1], slice - m.slices[0], b, h, part);
+    if (slice < m.slices[0]) move_rows<THREADS, uint4>(m, m.e.rows[0], m.lanes[0], slice, b, h, part);
+    else if (slice < m.slices[0] + m.slices[1]) move_rows<THREADS, uint4>(m, m.e.rows[1], m.lanes[1], slice - m.slices[0], b, h, part);
     else if (slice < m.slices[0] + m.slices[1] + m.slices[2])
-        move_rows<uint8_t>(m, m.e.rows[2], m.lanes[2], slice - m.slices[0] - m.slices[1], b, h, part);
-    else move_rows<uint8_t>(m, m.e.rows[3], m.lanes[3], slice - m.slices[0] - m.slices[1] - m.slices[2], b, h, part);
+        move_rows<THREADS, uint8_t>(m, m.e.rows[2], m.lanes[2], slice - m.slices[0] - m.slices[1], b, h, part);
+    else move_rows<THREADS, uint8_t>(m, m.e.rows[3], m.lanes[3], slice - m.slices[0] - m.slices[1] - m.slices[2], b, h, part);
 }
 
 }  // namespace
@@ -577,7 +578,9 @@ int launch_kv_evict(const EvictParams& p_in, int num_cus, hipStream_t stream) {
     // Slices of the rows: 256 bytes, if that gives two workgroups to a compute unit - then one launch does it, each workgroup
     // first the rows that depend on each other, then the rest (32 x 8 kv heads, 2048 rows of K and V kept: 114 us, with slices of
     // 128 bytes 126 us: the rate of a large copy).  Otherwise 128 bytes, and the rest in a launch of its own with more
-    // workgroups to a slice; short results stay one launch, which costs less than the few chunks it would spread.
+    // workgroups to a slice; short results stay one launch, which costs less than the few chunks it would spread.  The launch of
+    // the dependent rows alone has workgroups of 1024 threads, a quarter of the chunks that wait for one another (8 heads, 1024 such
+    // rows: 8.5 us, with 256 threads 12.7; one launch for 256 rows: 7.9 us, with 256 threads 6.1).
     const int64_t rows = (int64_t)p.batch * p.hkv;
     int slices = 0;
     bool one = false;
@@ -601,16 +604,17 @@ int launch_kv_evict(const EvictParams& p_in, int num_cus, hipStream_t stream) {
     m.parallel = one ? 1 : 0;
     m.parts = 1;
     m.row_blocks = slices;
-    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(slices + (one ? weight_blocks : 0)), (unsigned)p.hkv, (unsigned)p.batch), dim3(256),
-                       0, stream, m);
+    const dim3 grid((unsigned)(slices + (one ? weight_blocks : 0)), (unsigned)p.hkv, (unsigned)p.batch);
+    if (one) hipLaunchKernelGGL(evict_move_kernel<256>, grid, dim3(256), 0, stream, m);
+    else hipLaunchKernelGGL(evict_move_kernel<1024>, grid, dim3(1024), 0, stream, m);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || one) return (int)e;
     m.serial = 0;
     m.parallel = 1;
     m.parts = (int32_t)((4 * (int64_t)num_cus + slices * rows - 1) / (slices * rows));
     m.row_blocks = slices * m.parts;
-    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(m.row_blocks + weight_blocks), (unsigned)p.hkv, (unsigned)p.batch), dim3(256), 0,
-                       stream, m);
+    hipLaunchKernelGGL(evict_move_kernel<256>, dim3((unsigned)(m.row_blocks + weight_blocks), (unsigned)p.hkv, (unsigned)p.batch), dim3(256),
+                       0, stream, m);
     return (int)hipGetLastError();
 }
 
