@@ -78,6 +78,27 @@ def test_weights_of_lengths_and_pages(cuda_device, kind, d, page):
     _accumulate(kind, LENS, 8, 2, d, page, torch.bfloat16, d + page, cuda_device)
 
 
+@pytest.mark.parametrize("batch", [2, 63, 64, 65, 130])
+@pytest.mark.parametrize("kind,hkv", [("16bit", 1), ("mxfp4", 4)])
+def test_weights_of_ragged_batches(cuda_device, kind, hkv, batch):
+    """Tables that may hold long sequences: workgroups by length.  One long sequence, empty ones, ones of one token; many
+    alike; all empty."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 90, (batch,), generator=g).tolist()
+    lens[-1], lens[batch // 2], lens[0] = 2100, 0, 1
+    _accumulate(kind, lens, 2 * hkv, hkv, 64, 16, torch.bfloat16, batch, cuda_device)
+    _accumulate(kind, [lens[0]] + [300] * (batch - 2) + [2048], hkv, hkv, 64, 16, torch.float16, batch, cuda_device, length=2048)
+    q = torch.randn(batch, hkv, 64, device=cuda_device, dtype=torch.float16)
+    w = torch.rand(batch, hkv, 3200, device=cuda_device)
+    before = w.clone()
+    import triton_distributed_amd as tda
+    tda.accumulate_attention_weights(q, torch.zeros(1, 16, hkv, 64, device=cuda_device, dtype=torch.float16),
+                                     torch.zeros(batch, 200, dtype=torch.int32, device=cuda_device),
+                                     torch.zeros(batch, dtype=torch.int32, device=cuda_device),
+                                     torch.zeros(batch, hkv, device=cuda_device), 0.1, w)
+    assert torch.equal(w, before)
+
+
 @pytest.mark.parametrize("kind,d", [("16bit", 192), ("16bit", 576), ("fp8", 192), ("fp8", 576)])
 def test_weights_of_two_segment_rows(cuda_device, kind, d):
     _accumulate(kind, [300, 17, 0], 16, 1, d, 16, torch.float16, d, cuda_device)

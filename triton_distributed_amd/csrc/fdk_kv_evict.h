@@ -25,6 +25,7 @@ struct AttnWeightsParams {
     int32_t page_size, page_shift;           // page_shift = log2(page_size) or -1
     int32_t max_tokens;                      // min(table capacity, weights_len)
     int32_t shares, heads_per_wg;            // workgroups per (sequence, block of kv heads); heads of a block
+    int32_t balanced;                        // workgroups go to the sequences by their lengths: shares is the average
     float scale_log2, sm_scale, soft_cap;
 };
 
