@@ -207,7 +207,7 @@ __device__ __forceinline__ Level read_level(const EvictParams& p, int level, int
     const int word = bins / 2 - 1 - tid, top = 2 * word + 1;          // this thread's bins: top, top - 1
     int c0 = 0, c1 = 0, m0 = 0, m1 = 0;
     if (word >= 0) {
-#pragma unroll 8
+#pragma unroll 16
         for (int s = 0; s < p.segments; ++s) {
             const uint32_t x = segment_hist(p, level, seg0 + s)[word];
             c0 += (int)(x >> 16);
