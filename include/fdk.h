@@ -32,6 +32,12 @@
  *                        ModelBuilder.make_qk_norm_rope_update_kvcache, models/model_builder.py:341-379
  *                        (per-head RMSNorm of q and k, rotary embedding, K/V rows appended to the paged cache)
  *
+ * Without a counterpart in the reference (revision 3):
+ *   fdk_kv_append_axes   the append with explicit positions of one to four axes, and into MXFP4 caches
+ *   fdk_mx_quantize, fdk_mx_dequantize    16-bit rows to and from MXFP4 rows
+ *   fdk_accumulate_weights                what each cached token receives from a query's attention
+ *   fdk_kv_evict, fdk_kv_evict_workspace_bytes    the tokens with the least of it leave the cache
+ *
  * Conventions
  *   - Return value: 0 on success; a negative FDK_E* code when the arguments are rejected (nothing was
  *     launched); a positive value is the hipError_t of a failed launch.  Never exits the process.
@@ -211,8 +217,8 @@ typedef struct fdk_decode_args {
     int32_t reserved3;
 
     /* (revision 3) kv_dtype FDK_MXFP4: the scale bytes of the caches, [num_pages, P, Hkv, D/32], with byte strides of the
-     * page, token and head axes; rows aligned to 4 bytes (head_dim 64: 2).  k_scale / v_scale are not read.  Built for head_dim 64, 128 and 256 with
-     * v_head_dim = head_dim on the matrix-core path; no single-launch form; with counters, too, a forced split count runs as
+     * page, token and head axes; rows aligned to 4 bytes (head_dim 64: 2).  k_scale / v_scale are not read.  Built for
+     * head_dim 64, 128 and 256 with v_head_dim = head_dim on the matrix-core path; no single-launch form; with counters, too, a forced split count runs as
      * one workgroup per piece.  A value takes part as code * 2^(byte - 127) converted to q's dtype, exact within its range */
     const uint8_t* k_block_scale;
     const uint8_t* v_block_scale;

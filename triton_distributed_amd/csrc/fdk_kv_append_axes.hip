@@ -11,6 +11,9 @@
 // rounds of rows: prompts, whose rows outnumber the resident wavefronts, take four rounds (the loads of all of them are
 // requested together), single tokens one, which is the most wavefronts for the least latency.  A block of an MXFP4 row is the
 // values of eight neighbouring lanes.
+//
+// Prompts are bound by the bytes moved: 2 x 2041 tokens of 64 q and 8 kv heads, D = 128, into MXFP4 in 37 us (157 MB, 4.2 TB/s;
+// a large copy reaches 4.9); single tokens by launch and latency: 32 of them in 4.7 us, a smallest launch takes 4.4.
 #include "fdk_mxfp4.h"
 
 namespace fdk {
