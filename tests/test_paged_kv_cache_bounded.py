@@ -120,3 +120,29 @@ def test_a_serving_loop_at_a_budget(cuda_device, dtype):
     q = c.append(0, qkv.to(dev), wq.to(dev), wk.to(dev), cos.to(dev), sin.to(dev))
     want, pair = rope_axes.norm_rope(qkv[:, :, :hq], wq, 1e-6, cos, sin, torch.full((1, b, 1), seen), (d // 2,), False)
     assert ((q.cpu().double() - want).abs() <= 2.0 ** -7 * (pair + want.abs()) + 2.0 ** -20).all()
+
+
+@pytest.mark.gpu
+def test_eviction_and_append_on_another_stream(cuda_device):
+    """What the cache works out with torch goes with the kernels, while the current stream is busy with something else."""
+    dev = cuda_device
+    c = _cache(dev)
+    c.inc_offset(30)
+    w = torch.rand(2, 3, 2, 64, device=dev)
+    ang = torch.rand(200, 32, device=dev) * 6.28
+    qkv = torch.randn(3, 1, 8, 64, device=dev).bfloat16()
+    ones = torch.ones(64, device=dev, dtype=torch.bfloat16)
+    cos, sin = (torch.cat([t, t], -1) for t in (ang.cos(), ang.sin()))
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(int(2e7))
+    assert tuple(c.evict(w, 20, 5, stream=other).shape) == (2, 3, 2, 20)
+    with torch.cuda.stream(other):
+        c.inc_offset(1)
+    q = c.append(0, qkv, ones, ones, cos, sin, stream=other)
+    other.synchronize()
+    assert c.kv_lens.tolist() == [21] * 3
+    torch.cuda.synchronize()
+    assert c.next_positions(1).tolist() == [[30]] * 3
+    want = c.append(0, qkv, ones, ones, cos, sin, positions=torch.full((3, 1), 30, dtype=torch.int32, device=dev))
+    assert torch.equal(q, want)

@@ -848,7 +848,7 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
             x.positions = positions.data_ptr()
         if a.kv_dtype == _lib.FDK_MXFP4:
             x.k_block_scale, x.v_block_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        _lib.check(_LIB.fdk_kv_append_axes(C.byref(x), _stream_handle(stream)))
+        _launch_on(qkv.device, stream, _LIB.fdk_kv_append_axes, x)
         return q_norm_rope
     q_given = q_norm_rope is not None
     if qkv.dim() != 4 or key_cache.dim() != 4 or value_cache.dim() != 4:
@@ -944,7 +944,7 @@ def qk_norm_rope_update_kvcache(qkv: torch.Tensor, key_cache: torch.Tensor, valu
             x.pos_stride_axis, x.pos_stride_b, x.pos_stride_t = pos.stride()
             x.num_axes, x.rope_interleaved = axes, int(bool(rope_interleaved))
             x.rope_sections = (C.c_int32 * 4)(*sections)
-        _lib.check(_LIB.fdk_kv_append_axes(C.byref(x), _stream_handle(stream)))
+        _launch_on(qkv.device, stream, _LIB.fdk_kv_append_axes, x)
     else:
         _lib.check(_LIB.fdk_kv_append(C.byref(a), _stream_handle(stream)))
     # (only after the library has accepted the block; a result tensor of the call's own has the contiguous layout)

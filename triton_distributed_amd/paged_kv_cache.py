@@ -25,6 +25,7 @@ The class itself allocates with torch and launches nothing; it works on any torc
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -175,9 +176,17 @@ class PagedKVCache:
         k, v, table, lens = self.get_layer_kv_cache(layer_idx)
         ks, vs = self.layer_scales(layer_idx)
         if self._seen is not None and kwargs.get("positions") is None:
-            kwargs["positions"] = self.next_positions(qkv.shape[1])
+            with self._on(stream):
+                kwargs["positions"] = self.next_positions(qkv.shape[1])
         return qk_norm_rope_update_kvcache(qkv, k, v, table, lens, q_rms_weight, k_rms_weight, cos_cache, sin_cache,
                                            q_norm_rope, q_rms_eps, k_rms_eps, k_scale=ks, v_scale=vs, stream=stream, **kwargs)
+
+    def _on(self, stream):
+        """torch's work in line with the kernels on ``stream``: it reads and holds what they read and write."""
+        if stream is None:
+            return contextlib.nullcontext()
+        from .flash_decode import _on_stream, _stream_handle
+        return _on_stream(self.device, _stream_handle(stream))
 
     def next_positions(self, new_tokens: int) -> torch.Tensor:
         """Positions ``[B, T]`` int32 of the T tokens that ``inc_offset(T)`` has just counted: how many tokens their
@@ -202,9 +211,10 @@ class PagedKVCache:
             raise ValueError(f"weights must be [{self.num_layers}, B, Hkv, S] with S >= {self._host_len} tokens")
         if self._host_len <= keep:
             return None
-        kept = torch.empty((self.num_layers, self.batch_size, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
+        with self._on(stream):
+            kept = torch.empty((self.num_layers, self.batch_size, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
+            seen = self.kv_lens.clone() if self._seen is None else self._seen
         scales = {} if not self.mxfp4 else dict(k_scale=self.k_block_scale, v_scale=self.v_block_scale)
-        seen = self.kv_lens.clone() if self._seen is None else self._seen
         for layer in range(self.num_layers):
             # (the layers share kv_lens: the last one changes it)
             lens_out = self.kv_lens if layer == self.num_layers - 1 else None
