@@ -413,7 +413,7 @@ typedef struct fdk_kv_evict_args {
     int32_t batch, num_kv_heads, head_dim, v_head_dim; /* v_head_dim 0: head_dim */
     int32_t page_size, max_pages, weights_len;
     int32_t keep, recent;       /* 0 <= recent <= keep, 1 <= keep <= weights_len */
-    int32_t reserved1;
+    int32_t num_pages;          /* of the pool: rows of pages outside it are left out */
 } fdk_kv_evict_args;
 
 struct fdk_measure_args; /* include/fdk_measure.h */

@@ -320,3 +320,30 @@ def test_another_stream_than_the_current_one(cuda_device):
     rows, want_new, want_kept, want_w = okv.evict([c["k"], c["v"]], table, [400], w, 100, 20)
     assert torch.equal(new.cpu(), want_new) and torch.equal(kept.cpu(), want_kept) and torch.equal(wo.cpu(), want_w)
     assert torch.equal(k.cpu(), rows[0]) and torch.equal(v.cpu(), rows[1])
+
+
+@pytest.mark.parametrize("kind", ["16bit", "mxfp4"])
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 12, 2 ** 31 - 1])
+def test_rows_of_pages_outside_the_pool_are_left_out(cuda_device, kind, bad):
+    """64 tokens on four pages, the last 32 stay: a source page and, in another sequence, a target page that the pool of
+    12 does not have."""
+    import triton_distributed_amd as tda
+    dev, shape = cuda_device, (12, 16, 2, 64)
+    g = torch.Generator().manual_seed(3)
+    if kind == "mxfp4":
+        pools = [torch.randint(0, 256, shape[:3] + (n,), dtype=torch.uint8, generator=g) for n in (32, 32, 2, 2)]
+    else:
+        pools = [torch.randn(shape, generator=g).bfloat16() for _ in range(2)]
+    table = torch.tensor([[3, 5, bad, 7], [1, bad, 0, 2], [4, 6, 8, 9]], dtype=torch.int32)
+    want = [t.clone() for t in pools]
+    for t, before in zip(want, pools):
+        t[5] = before[7]                       # (slots 0 .. 15 of sequence 0 would come from the bad page)
+        t[1] = before[0]                       # (slots 16 .. 31 of sequence 1 would go to it)
+        t[4], t[6] = before[8], before[9]
+    got = [t.to(dev) for t in pools]
+    weights = torch.arange(64, dtype=torch.float32, device=dev).expand(3, 2, 64).contiguous()
+    scales = dict(k_scale=got[2], v_scale=got[3]) if kind == "mxfp4" else {}
+    lens, kept, _ = tda.evict_kvcache(got[0], got[1], table.to(dev), torch.full((3,), 64, dtype=torch.int32, device=dev), weights, 32, 4, **scales)
+    assert lens.tolist() == [32] * 3 and kept[0, 0].tolist() == list(range(32, 64))
+    for t, w in zip(got, want):
+        assert torch.equal(t.cpu(), w)

@@ -58,7 +58,7 @@ def _evict_args(**kw):
     a.weights_out, a.weights_out_stride_b, a.weights_out_stride_h = 0x60000, 8 * 4096, 4096
     a.kept, a.kv_lens_out, a.workspace, a.workspace_bytes = 0x70000, 0x80000, 0x90000, 32 * 8 * 16
     a.batch, a.num_kv_heads, a.head_dim = 32, 8, 128
-    a.page_size, a.max_pages, a.weights_len, a.keep, a.recent = 16, 256, 4096, 2048, 256
+    a.page_size, a.max_pages, a.weights_len, a.keep, a.recent, a.num_pages = 16, 256, 4096, 2048, 256, 8192
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -68,7 +68,7 @@ def _evict_args(**kw):
     ({}, 0), (dict(batch=0, k_cache=None), 0), (dict(weights_out=0x50000, kv_lens_out=0x40000), 0), (dict(keep=4096, recent=4096), 0),
     (dict(kv_dtype=_lib.FDK_FP8_E4M3), 0), (dict(struct_size=16), _lib.FDK_EABI), (dict(kv_dtype=_lib.FDK_FP32), _lib.FDK_EUNSUPPORTED),
     (dict(kv_dtype=_lib.FDK_MXFP4), _lib.FDK_ENULL), (dict(head_dim=40), _lib.FDK_EUNSUPPORTED), (dict(v_head_dim=8192), _lib.FDK_EUNSUPPORTED),
-    (dict(keep=0), _lib.FDK_ESHAPE), (dict(keep=4097), _lib.FDK_ESHAPE), (dict(recent=-1), _lib.FDK_ESHAPE), (dict(recent=2049), _lib.FDK_ESHAPE),
+    (dict(keep=0), _lib.FDK_ESHAPE), (dict(keep=4097), _lib.FDK_ESHAPE), (dict(num_pages=0), _lib.FDK_ESHAPE), (dict(recent=-1), _lib.FDK_ESHAPE), (dict(recent=2049), _lib.FDK_ESHAPE),
     (dict(v_cache=0x20008), _lib.FDK_EALIGN), (dict(v_cache=None), _lib.FDK_ENULL), (dict(kept=None), _lib.FDK_ENULL),
     (dict(weights_out=None), _lib.FDK_ENULL), (dict(kv_lens_out=None), _lib.FDK_ENULL), (dict(workspace=None), _lib.FDK_EWORKSPACE),
     (dict(workspace_bytes=32 * 8 * 16 - 1), _lib.FDK_EWORKSPACE), (dict(workspace=0x90008), _lib.FDK_EALIGN), (dict(kept=0x70001), _lib.FDK_EALIGN),

@@ -122,7 +122,7 @@ def _conv(**kw):
     (dict(x=0), _lib.FDK_ENULL), (dict(x=0x10008), _lib.FDK_EALIGN), (dict(codes=0x20002), _lib.FDK_EALIGN),
     (dict(x_stride=(C.c_int64 * 3)(0, 0, 132)), _lib.FDK_EALIGN), (dict(codes_stride=(C.c_int64 * 3)(0, 0, 66)), _lib.FDK_EALIGN),
     (dict(n=(C.c_int32 * 3)(1, -1, 1)), _lib.FDK_ESHAPE), (dict(n=(C.c_int32 * 3)(0, 1, 1), x=0), 0),
-    (dict(n=(C.c_int32 * 3)(2 ** 31 - 1, 2 ** 31 - 1, 4)), _lib.FDK_ESHAPE), (dict(struct_size=8), _lib.FDK_EABI),
+    (dict(n=(C.c_int32 * 3)(2 ** 31 - 1, 2 ** 31 - 1, 4)), _lib.FDK_ESHAPE), (dict(n=(C.c_int32 * 3)(2 ** 20, 2 ** 10, 4)), _lib.FDK_ESHAPE), (dict(struct_size=8), _lib.FDK_EABI),
 ])
 def test_conversion_refusals(kw, code):
     lib = _lib.load()

@@ -165,7 +165,7 @@ class FdkKvEvictArgs(C.Structure):
         ("kept", C.c_void_p), ("kv_lens_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("batch", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("v_head_dim", C.c_int32),
         ("page_size", C.c_int32), ("max_pages", C.c_int32), ("weights_len", C.c_int32),
-        ("keep", C.c_int32), ("recent", C.c_int32), ("reserved1", C.c_int32),
+        ("keep", C.c_int32), ("recent", C.c_int32), ("num_pages", C.c_int32),
     ]
 
 

@@ -862,7 +862,8 @@ static int mxfp4_convert(const fdk_mxfp4_args* caller_args, bool quantize, void*
     if (a->num_values <= 0 || a->num_values % fdk::kMxBlock) return fail(FDK_ESHAPE, "num_values %d: a positive multiple of 32", a->num_values);
     if (a->x_dtype != FDK_BF16 && a->x_dtype != FDK_FP16) return fail(FDK_EUNSUPPORTED, "x_dtype %d (bf16 or fp16 only)", a->x_dtype);
     if (!a->n[0] || !a->n[1] || !a->n[2]) return FDK_OK;
-    if ((unsigned __int128)a->n[0] * a->n[1] * a->n[2] * (a->num_values / 8) > (unsigned __int128)INT32_MAX * 256)
+    // (a thread per eight values; a launch holds less than 2^32)
+    if ((unsigned __int128)a->n[0] * a->n[1] * a->n[2] * (a->num_values / 8) > (unsigned __int128)UINT32_MAX - 255)
         return fail(FDK_ESHAPE, "too many rows");
     if (!a->x || !a->codes || !a->scales) return fail(FDK_ENULL, "x / codes / scales must be non-null");
     for (int i = 0; i < 3; ++i) {
@@ -1128,6 +1129,7 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     if (a->weights_len <= 0) return fail(FDK_ESHAPE, "weights_len %d <= 0", a->weights_len);
     if (a->keep < 1 || a->keep > a->weights_len) return fail(FDK_ESHAPE, "keep %d outside [1, weights_len = %d]", a->keep, a->weights_len);
     if (a->recent < 0 || a->recent > a->keep) return fail(FDK_ESHAPE, "recent %d outside [0, keep = %d]", a->recent, a->keep);
+    if (a->num_pages <= 0) return fail(FDK_ESHAPE, "num_pages %d <= 0", a->num_pages);
     if (a->batch == 0) return FDK_OK;
     if (int rc = check_pages(a->batch, a->page_size, a->max_pages, a->table_stride_b, a->block_table, a->kv_lens)) return rc;
     const int kb = mx ? a->head_dim / 2 : a->head_dim * es, vb = mx ? dv / 2 : dv * es;
@@ -1173,6 +1175,7 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     p.batch = a->batch; p.hkv = a->num_kv_heads; p.keep = a->keep; p.recent = a->recent;
     p.weights_len = a->weights_len;
     p.max_tokens = evict_max_tokens(a);
+    p.num_pages = a->num_pages;
     p.page_size = a->page_size; p.page_shift = ilog2_exact(a->page_size);
     const int rc = fdk::launch_kv_evict(p, query_cus(), reinterpret_cast<hipStream_t>(hip_stream));
     if (rc) return fail(rc, "eviction launch failed: %s", hipGetErrorString((hipError_t)rc));

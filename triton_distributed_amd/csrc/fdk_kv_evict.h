@@ -49,7 +49,7 @@ struct EvictParams {
     int32_t batch, hkv, keep, recent;
     int32_t weights_len, max_tokens;
     int32_t page_size, page_shift;
-    int32_t num_tensors;
+    int32_t num_tensors, num_pages;
     // rows whose weights are spread over several workgroups (parts of the workspace)
     int32_t segments;
     int2* row_state;                         // [rows][2]: leading bits of the last survivor's weight, survivors left to find

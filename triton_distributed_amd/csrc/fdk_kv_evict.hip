@@ -463,14 +463,19 @@ __device__ __forceinline__ void move_rows(const MoveParams& m, const EvictRows& 
 #pragma unroll
         for (int u = 0; u < U; ++u) pg[u] = tbl[place(src[u])];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = load_row(reinterpret_cast<const V*>(base + pg[u] * r.sp + slot(src[u]) * r.st));
+        for (int u = 0; u < U; ++u) {
+            const bool inside = (uint32_t)pg[u] < (uint32_t)p.num_pages && (uint32_t)pg_to[u] < (uint32_t)p.num_pages;
+            if (!inside) pg[u] = 0;
+            if (!inside) pg_to[u] = -1;                    // (not stored)
+            x[u] = load_row(reinterpret_cast<const V*>(base + pg[u] * r.sp + slot(src[u]) * r.st));
+        }
 #pragma unroll
-        for (int u = 0; u < U; ++u) to[u] = base + pg_to[u] * r.sp + slot(min(j0 + u * rows + row, end - 1)) * r.st;
+        for (int u = 0; u < U; ++u) to[u] = pg_to[u] < 0 ? nullptr : base + pg_to[u] * r.sp + slot(min(j0 + u * rows + row, end - 1)) * r.st;
     };
     auto write = [&](int j0, int end) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (j0 + u * rows + row < end) store_row(reinterpret_cast<V*>(to[u]), x[u]);
+            if (j0 + u * rows + row < end && to[u]) store_row(reinterpret_cast<V*>(to[u]), x[u]);
     };
     if (m.serial) {
         for (int j0 = plan.x; j0 < plan.y; j0 += chunk) {

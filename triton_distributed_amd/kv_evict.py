@@ -143,6 +143,9 @@ def evict_kvcache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tabl
     block_table  [B, max_pages] int32, kv_lens [B] int32, weights [B, Hkv, S] fp32 with S covering every length
     keep, recent 1 <= keep <= S, 0 <= recent <= keep; a sequence of at most ``keep`` tokens stays as it is
 
+    Rows move within a sequence's own pages: no other sequence may share them.  (A row that would come from or go to a page number
+    outside the pool is left out.)
+
     Returns ``(kv_lens_out [B] int32 = min(kv_lens, keep), kept [B, Hkv, keep] int32, weights_out [B, Hkv, S])``: ``kept`` is
     the slot that the token in each slot had before (-1 behind the new length), ``weights_out`` the survivors' weights and 0
     behind them.  ``weights_out`` may be ``weights`` and ``kv_lens_out`` may be ``kv_lens``.  Rows behind the new length keep
@@ -190,7 +193,7 @@ def evict_kvcache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tabl
         a.weights_stride_b, a.weights_stride_h = weights.stride(0), weights.stride(1)
         a.batch, a.num_kv_heads, a.head_dim, a.v_head_dim = batch, kv_heads, _row_values(key_cache), _row_values(value_cache)
         a.page_size, a.max_pages, a.weights_len = key_cache.shape[1], block_table.shape[1], length
-        a.keep, a.recent = keep, recent
+        a.keep, a.recent, a.num_pages = keep, recent, key_cache.shape[0]
         a.workspace_bytes = _LIB.fdk_kv_evict_workspace_bytes(C.byref(a))
     if stream is None:
         weights_out, kv_lens_out, kept, buf = _evict_buffers(weights, kv_lens, keep, weights_out, kv_lens_out, kept, a.workspace_bytes)
