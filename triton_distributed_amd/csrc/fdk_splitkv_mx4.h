@@ -17,7 +17,12 @@
 //       halves of the step (K rows are assigned to the rows of S^T that way, so that one V load instruction reads four
 //       consecutive tokens).
 // The 64-byte rows of two kv heads share a 128-byte line, and so do the scales of four tokens and all heads: every unit of a
-// (sequence, split) runs on one XCD, with loads that leave the lines in its L2 (tiles_on_one_xcd).
+// (sequence, split) runs on one XCD, with loads that leave the lines in its L2 (tiles_on_one_xcd).  Pairs of 64-byte rows with
+// pages of 16 << n tokens go through LDS instead (fdk_splitkv_mx4_staged.hip).
+//
+// Bound by the bytes of the rows, laid out by head: 4 sequences x 8 kv heads x 131072 tokens (570 MB) in 91 us, 6.3 TB/s; 32 x 8 x 4096
+// (143 MB) in 27 us, 5.3 TB/s, fill and drain included.  The arithmetic (96 conversions and permutes, 16 MFMAs and a softmax of a step
+// of 32 tokens) is about half of that time by its instructions' rates, and runs beside the loads.
 #pragma once
 
 #include "fdk_mxfp4.h"
