@@ -215,3 +215,55 @@ def test_captured_and_replayed_on_another_stream(cuda_device):
         _close(call.out, o64, tol_o)
         _close(call.lse, l64, tol_l)
         assert math.isfinite(float(call.out.float().sum()))
+
+
+@pytest.mark.parametrize("d,page,hkv", [(128, 16, 2), (128, 16, 1), (128, 24, 2), (64, 16, 2), (256, 16, 2)])
+def test_pages_past_32_bit_offsets(cuda_device, d, page, hkv):
+    """Pools of which most pages lie more than 4 GiB behind the first: append, decode, attention weights and eviction leave
+    the same bits as on the same pages side by side."""
+    import triton_distributed_amd as tda
+    dev, pages, far = cuda_device, 12, 700 << 20
+    buf = torch.empty(pages * far, dtype=torch.uint8, device=dev)
+    shapes = [(pages, page, hkv, n) for n in (d // 2, d // 2, d // 32, d // 32)]
+    at = (0, 200 << 20, 400 << 20, 500 << 20)
+    wide = [torch.as_strided(buf, s, (far, hkv * s[3], s[3], 1), o) for s, o in zip(shapes, at)]
+    g = torch.Generator().manual_seed(d + page)
+    near = [torch.randint(0, 256, s, dtype=torch.uint8, generator=g).to(dev) for s in shapes[:2]]
+    near += [torch.randint(118, 130, s, dtype=torch.uint8, generator=g).to(dev) for s in shapes[2:]]
+    for w, n in zip(wide, near):
+        w.copy_(n)
+    table = torch.randperm(pages, generator=g).to(torch.int32).view(2, 6).to(dev)
+    lens = torch.tensor([6 * page - 3, 2 * page + 5], dtype=torch.int32, device=dev)
+    ang = torch.rand(300, d // 2, generator=g) * 6.28
+    cos, sin = (torch.cat((t, t), -1).to(dev) for t in (ang.cos(), ang.sin()))
+    ones = torch.ones(d, dtype=torch.bfloat16, device=dev)
+    qkv = torch.randn(2, 4, 6 * hkv, d, generator=g).bfloat16().to(dev)
+    got = []
+    for k, v, ks, vs in (near, wide):
+        q = tda.qk_norm_rope_update_kvcache(qkv, k, v, table, lens, ones, ones, cos, sin, k_scale=ks, v_scale=vs)[:, -1]
+        out, lse = tda.flash_decode(q, k, v, table, lens, 0.1, k_scale=ks, v_scale=vs)
+        w = tda.accumulate_attention_weights(q, k, table, lens, lse, 0.1, torch.zeros(2, hkv, 6 * page, device=dev), k_scale=ks)
+        n, kept, w2 = tda.evict_kvcache(k, v, table, lens, w, 2 * page, 7, k_scale=ks, v_scale=vs)
+        got.append([q, out, lse, w, n, kept, w2, k, v, ks, vs])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert torch.isfinite(got[0][1]).all() and int(got[0][4][0]) == 2 * page
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 7), (256, 32)])
+def test_scales_and_rows_laid_out_apart(cuda_device, d, page):
+    """Block scales in the middle of wider rows, tokens with room between them: the same bits as side by side."""
+    import triton_distributed_amd as tda
+    lens, hkv, hq = [300, 1, 77], 2, 6
+    (kc, ks, _, vc, vs, _), table = make_cache(lens, page, hkv, d, torch.bfloat16, d)
+    dev = [t.to(cuda_device) for t in (kc, vc, ks, vs)]
+    apart = []
+    for i, t in enumerate(dev):
+        room = torch.full(t.shape[:2] + (hkv + 2, t.shape[3] + (0 if i < 2 else 8)), 0xFF, dtype=torch.uint8, device=cuda_device)
+        view = room[:, :, 1:1 + hkv, :t.shape[3]] if i < 2 else room[:, :, 1:1 + hkv, 4:4 + t.shape[3]]
+        apart.append(view.copy_(t))
+    q = torch.randn(3, hq, d, generator=torch.Generator().manual_seed(1)).bfloat16().to(cuda_device)
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    for kw in ({}, dict(kv_split=3), dict(force_balanced=True)):
+        a, b = (tda.flash_decode(q, k, v, table.to(cuda_device), n, 0.1, k_scale=s, v_scale=t, **kw) for k, v, s, t in (dev, apart))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
