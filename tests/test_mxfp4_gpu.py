@@ -267,3 +267,25 @@ def test_scales_and_rows_laid_out_apart(cuda_device, d, page):
     for kw in ({}, dict(kv_split=3), dict(force_balanced=True)):
         a, b = (tda.flash_decode(q, k, v, table.to(cuda_device), n, 0.1, k_scale=s, v_scale=t, **kw) for k, v, s, t in (dev, apart))
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 5)])
+def test_scales_of_a_head_past_32_bit_offsets(cuda_device, d, page):
+    """Block scales laid out by head, the second head's more than 4 GiB behind the first's."""
+    import triton_distributed_amd as tda
+    lens, hkv = [90, 33], 2
+    (kc, ks, _, vc, vs, _), table = make_cache(lens, page, hkv, d, torch.float16, d)
+    k, v, ks, vs, table = (t.to(cuda_device) for t in (kc, vc, ks, vs, table))
+    buf = torch.empty((4 << 30) + (64 << 20), dtype=torch.uint8, device=cuda_device)
+    far = [torch.as_strided(buf, t.shape, (page * d // 32, d // 32, (4 << 30) + 256, 1), o).copy_(t) for t, o in ((ks, 0), (vs, 32 << 20))]
+    q = torch.randn(2, 6, d, generator=torch.Generator().manual_seed(1)).half().to(cuda_device)
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda_device)
+    got = []
+    for s, t in ((ks, vs), far):
+        out, lse = tda.flash_decode(q, k, v, table, n, 0.1, k_scale=s, v_scale=t)
+        got.append([out, lse, tda.accumulate_attention_weights(q, k, table, n, lse, 0.1, torch.zeros(2, hkv, 90, device=cuda_device), k_scale=s)])
+        kk, vv = k.clone(), v.clone()
+        tda.evict_kvcache(kk, vv, table, n, got[-1][-1], 20, 5, k_scale=s, v_scale=t)
+        got[-1] += [kk, vv, s, t]
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

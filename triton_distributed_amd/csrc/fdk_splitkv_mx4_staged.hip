@@ -108,12 +108,12 @@ __global__ __launch_bounds__(512) void splitkv_mx4_staged_kernel(const SplitPara
     const float inv_cap = p.soft_cap > 0.f ? 1.0f / p.soft_cap : 0.f;
     const char* kplane = reinterpret_cast<const char*>(p.k) + (int64_t)kvh0 * p.k_sh;
     const char* vplane = reinterpret_cast<const char*>(p.v) + (int64_t)kvh0 * p.v_sh;
-    const char* ksplane = reinterpret_cast<const char*>(x.k) + (int64_t)kvh0 * x.k_sh;
-    const char* vsplane = reinterpret_cast<const char*>(x.v) + (int64_t)kvh0 * x.v_sh;
+    const char* ksplane = reinterpret_cast<const char*>(x.k) + (int64_t)(kvh0 + sc_head) * x.k_sh;      // (of this lane's head)
+    const char* vsplane = reinterpret_cast<const char*>(x.v) + (int64_t)(kvh0 + sc_head) * x.v_sh;
     // this lane's byte offsets from the first token of an instruction
     const uint32_t krows = (uint32_t)tok8 * (uint32_t)p.k_st, vrows = (uint32_t)tok8 * (uint32_t)p.v_st;
-    const uint32_t kscales = (uint32_t)(sc_tok & 15) * (uint32_t)x.k_st + (uint32_t)sc_head * (uint32_t)x.k_sh;
-    const uint32_t vscales = (uint32_t)(sc_tok & 15) * (uint32_t)x.v_st + (uint32_t)sc_head * (uint32_t)x.v_sh;
+    const uint32_t kscales = (uint32_t)(sc_tok & 15) * (uint32_t)x.k_st;
+    const uint32_t vscales = (uint32_t)(sc_tok & 15) * (uint32_t)x.v_st;
 
     struct Pages { int32_t pg[2]; };           // of a step's two tiles of 16 tokens; positions past the piece stand for its last
     auto fetch_pages = [&](int t, Pages& pi) {
@@ -161,8 +161,8 @@ __global__ __launch_bounds__(512) void splitkv_mx4_staged_kernel(const SplitPara
         const bool second = sc_tok >= 16;                             // the tile of this lane's token
         if constexpr (CLAMP) {
             const int n = min(tok0 + sc_tok, last), pg = second ? pi.pg[1] : pi.pg[0];
-            scale_load(ksplane + offset(x.k_sp, x.k_st, pg, n & pmask) + (uint32_t)sc_head * (uint32_t)x.k_sh, kd);
-            scale_load(vsplane + offset(x.v_sp, x.v_st, pg, n & pmask) + (uint32_t)sc_head * (uint32_t)x.v_sh, vd);
+            scale_load(ksplane + offset(x.k_sp, x.k_st, pg, n & pmask), kd);
+            scale_load(vsplane + offset(x.v_sp, x.v_st, pg, n & pmask), vd);
         } else {
             const uint64_t k0 = offset(x.k_sp, x.k_st, pi.pg[0], tok0 & pmask), k1 = offset(x.k_sp, x.k_st, pi.pg[1], (tok0 + 16) & pmask);
             const uint64_t v0 = offset(x.v_sp, x.v_st, pi.pg[0], tok0 & pmask), v1 = offset(x.v_sp, x.v_st, pi.pg[1], (tok0 + 16) & pmask);
