@@ -146,3 +146,43 @@ def test_eviction_and_append_on_another_stream(cuda_device):
     assert c.next_positions(1).tolist() == [[30]] * 3
     want = c.append(0, qkv, ones, ones, cos, sin, positions=torch.full((3, 1), 30, dtype=torch.int32, device=dev))
     assert torch.equal(q, want)
+
+
+@pytest.mark.gpu
+def test_two_caches_at_once_on_two_streams_and_threads(cuda_device):
+    """The loop of two caches on two streams, from two threads, gives the bits that each gives by itself."""
+    import threading
+    dev = cuda_device
+    ang = torch.rand(400, 64, generator=torch.Generator().manual_seed(9)) * 6.28
+    cos, sin = (torch.cat([t, t], -1).to(dev) for t in (ang.cos(), ang.sin()))
+    ones = torch.ones(128, device=dev, dtype=torch.bfloat16)
+    prompts = [torch.randn(4, 300, 12, 128, generator=torch.Generator().manual_seed(i)).bfloat16().to(dev) for i in range(2)]
+    steps = [torch.randn(24, 4, 1, 12, 128, generator=torch.Generator().manual_seed(7 + i)).bfloat16().to(dev) for i in range(2)]
+    torch.cuda.synchronize()
+
+    def loop(i, got):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            c = PagedKVCache(PAGE_SIZE=16, num_layers=1, batch_size=4, max_length=400, num_kv_heads=2, head_dim=128,
+                             dtype=torch.float4_e2m1fn_x2, device=dev, generator=torch.Generator().manual_seed(i))
+            w = torch.zeros(1, 4, 2, 400, device=dev)
+            for x in [prompts[i], *steps[i]]:
+                c.inc_offset(x.shape[1])
+                q = c.append(0, x, ones, ones, cos, sin)[:, -1].contiguous()
+                out, lse = c.decode(0, q, 0.09)
+                c.accumulate(0, q, lse, 0.09, w[0])
+                got += [out, lse, w.clone()]
+                if c.max_kv_len > 200 + 4 * i:
+                    got.append(c.evict(w, 190, 30))
+            torch.cuda.current_stream().synchronize()
+    alone, together = ([], []), ([], [])
+    for i in range(2):
+        loop(i, alone[i])
+    threads = [threading.Thread(target=loop, args=(i, together[i])) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, together):
+        assert len(a) == len(b) > 75
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
