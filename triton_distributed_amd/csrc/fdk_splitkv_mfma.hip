@@ -46,7 +46,7 @@ bool mfma_supported(int q_dtype, int kv_dtype, int /*group*/, int head_dim, int 
 // 115 us).  e4m3 caches, whose values have to be converted on the way: from 17 q heads on (8 / 16 / 32 q heads: 52 / 53 /
 // 58 us against 50 / 52 / 90 us).
 int mfma_heads_per_wg(int group, int row_values, int kv_dtype) {
-    return row_values > 512 && kv_dtype != FDK_MXFP4 && (kv_dtype != FDK_FP8_E4M3 || group > 16) ? 64 : 16;
+    return row_values > 512 && (kv_dtype != FDK_FP8_E4M3 || group > 16) ? 64 : 16;
 }
 
 // kv heads per workgroup.  Adjacent kv heads of a token are adjacent in the cache, so a workgroup that takes
@@ -61,7 +61,6 @@ int mfma_heads_per_wg(int group, int row_values, int kv_dtype) {
 // (Rows of more than 512 values per token and kv head, K and V together: at most two heads, i.e. the four wavefronts
 // that the registers and the LDS of a compute unit hold at that size.)
 int mfma_kv_heads_per_wg(int batch, int hkv, int group, int num_cus, int row_values, int kv_dtype) {
-    if (kv_dtype == FDK_MXFP4) return 1;                                 // (fdk_splitkv_mx4.h)
     if (mfma_heads_per_wg(group, row_values, kv_dtype) > 16) return 1;   // the shared-tile kernels: one kv head, 64 q heads
     const int head_tiles = (group + 15) / 16;
     for (int nh = row_values > 512 ? 2 : 8; nh >= 1; nh >>= 1) {
