@@ -263,8 +263,6 @@ __global__ __launch_bounds__(64 * kWaves) void attn_weights_kernel(const AttnWei
         if (lane < 16 * TILES && mine < end) {
             float x = sum[0];
             if (TILES >= 2 && a == 1) x = sum[TILES >= 2 ? 1 : 0];
-            if (TILES == 4 && a == 2) x = sum[TILES == 4 ? 2 : 0];
-            if (TILES == 4 && a == 3) x = sum[TILES == 4 ? 3 : 0];
             wrow[mine] = r.old + x;
         }
     };
