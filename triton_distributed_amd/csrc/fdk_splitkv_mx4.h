@@ -13,7 +13,7 @@
 //   V   lane (c, a) loads values (D/16) c .. + D/16 - 1 of the tokens whose probabilities the lane group a holds, converts
 //       them (again with the scale of its own block) and pairs the tokens up with byte permutes: operand A of
 //       O^T += V^T P^T, row m = c of column block db being value (D/16) c + db.
-//   P   straight from the softmax registers: lane (h, a) holds the logits of head h for tokens a, a + 4, a + 8, a + 12 of both
+//   P   in two 16-bit parts, straight from the softmax registers: lane (h, a) holds the logits of head h for tokens a, a + 4, a + 8, a + 12 of both
 //       halves of the step (K rows are assigned to the rows of S^T that way, so that one V load instruction reads four
 //       consecutive tokens).
 // The 64-byte rows of two kv heads share a 128-byte line, and so do the scales of four tokens and all heads: every unit of a
@@ -49,7 +49,7 @@ struct Mx4Tile {                           // one step in registers, as loaded
 
 // What a wavefront does with a step of 32 tokens of one kv head, and how the wavefronts of a head are merged.  Lane (c, a):
 // q head c of the tile, tokens 16 hf + a + 4 i of the step.
-template <int QDT, int D>
+template <int QDT, int D, bool FOLDED>
 struct Mx4Math {
     using P2 = Pack2<QDT>;
     using T = Mx4Tile<D>;
@@ -92,11 +92,24 @@ struct Mx4Math {
         }
     }
 
-    // ---- online softmax for head c over this lane group's eight tokens; the probabilities as operand B of P V.  MASKED: only
+    // Eight probabilities as operand B of P V: rounded to 16 bits, and what that left over, rounded in turn: together within 2^-16
+    // (fp16: 2^-22) of them, so that the result is rounded once, when it is stored.  (The rounded ones alone are off by half a
+    // step of 16 bits, as much as the result's own rounding.)  FOLDED (groups of at most eight q heads): the columns c + 8 of
+    // every operand, which would be empty, stand for the heads c once more and take the second part: no matrix instruction is
+    // added, and O is the sum of columns c and c + 8 (leave_part).  Larger groups multiply V twice.  In us, the rounded ones
+    // alone / folded / V twice: 4 x 8 kv heads x 131072 tokens in token layout 105.7 / 106.8 / 110.4, by head 94.0 / 97.1 /
+    // 101.2; 32 x 8 x 4096 35.7 / 37.1 / 37.8, by head 27.2 / 27.4 / 28.8.
+    struct Probs {
+        uint4 hi, lo;
+    };
+    // the q head of the tile that column c stands for (columns without one repeat the last, and are not stored)
+    static __device__ __forceinline__ int head_of(int c, int heads_here) { return min(FOLDED ? c & 7 : c, heads_here - 1); }
+
+    // ---- online softmax for head c over this lane group's eight tokens.  MASKED: only
     // the first `left` tokens of the step (at least one) take part ----
     template <typename MaskedTag>
-    static __device__ __forceinline__ uint4 softmax(float (&sv)[8], float& m_run, float& l_run, f32x4_t (&acc)[DB], const SplitParams& p,
-                                                    float inv_cap, int a, int left, MaskedTag) {
+    static __device__ __forceinline__ Probs softmax(float (&sv)[8], float& m_run, float& l_run, f32x4_t (&acc)[DB], const SplitParams& p,
+                                                    float inv_cap, int a, int c, int left, MaskedTag) {
         if (p.soft_cap > 0.f) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sv[i] = soft_cap_fn(sv[i] * p.sm_scale, p.soft_cap, inv_cap) * kLog2e;
@@ -128,12 +141,21 @@ struct Mx4Math {
 #pragma unroll
         for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(sv[i] - m_run);
         l_run += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-        // probabilities rounded to the q dtype, as the 16-bit kernels do; the sum above is of the unrounded ones
-        return make_uint4(P2::pack(pr[0], pr[1]), P2::pack(pr[2], pr[3]), P2::pack(pr[4], pr[5]), P2::pack(pr[6], pr[7]));
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = P2::pack(pr[2 * i], pr[2 * i + 1]);
+            lo[i] = P2::pack(pr[2 * i] - P2::lo(hi[i]), pr[2 * i + 1] - P2::hi(hi[i]));
+        }
+        if constexpr (FOLDED) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) hi[i] = c >= 8 ? lo[i] : hi[i];
+        }
+        return Probs{make_uint4(hi[0], hi[1], hi[2], hi[3]), make_uint4(lo[0], lo[1], lo[2], lo[3])};
     }
 
     // ---- O^T[value][head] += V^T P^T ----
-    static __device__ __forceinline__ void values(const T& r, const uint4 pv, f32x4_t (&o)[DB]) {
+    static __device__ __forceinline__ void values(const T& r, const Probs& pv, f32x4_t (&o)[DB]) {
         float sc[8];
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) v_scales(r.vs[hf], sc + 4 * hf);
@@ -148,8 +170,13 @@ struct Mx4Math {
                 lo[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x05040100u);
                 hi[j] = __builtin_amdgcn_perm(u[2 * j + 1], u[2 * j], 0x07060302u);
             }
-            o[db] = mma(make_uint4(lo[0], lo[1], lo[2], lo[3]), pv, o[db]);
-            o[db + 1] = mma(make_uint4(hi[0], hi[1], hi[2], hi[3]), pv, o[db + 1]);
+            const uint4 v0 = make_uint4(lo[0], lo[1], lo[2], lo[3]), v1 = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            o[db] = mma(v0, pv.hi, o[db]);
+            o[db + 1] = mma(v1, pv.hi, o[db + 1]);
+            if constexpr (!FOLDED) {
+                o[db] = mma(v0, pv.lo, o[db]);
+                o[db + 1] = mma(v1, pv.lo, o[db + 1]);
+            }
         };
 #pragma unroll
         for (int w = 0; w < T::VW; ++w) {
@@ -165,8 +192,15 @@ struct Mx4Math {
     // A wavefront's part of the merge: block e = i (DB / 4) + q of its D * 64 bytes holds, per lane, the values
     // DB (4 a + i) + 4 q .. + 3 of head c - every LDS instruction touches one contiguous kilobyte, and a merging lane stores
     // four consecutive values -; m and l: [16]
-    static __device__ __forceinline__ void leave_part(const f32x4_t (&acc)[DB], float m_run, float l_run, char* part, float* m, float* l,
-                                                      bool live, int lane) {
+    static __device__ __forceinline__ void leave_part(f32x4_t (&acc)[DB], float m_run, float l_run, char* part, float* m, float* l,
+                                                      int heads_here, int lane) {
+        const bool live = (lane & 15) < heads_here;
+        if constexpr (FOLDED) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[db][i] += dpp_mov<0x128>(acc[db][i]);              // row_ror:8: the lane of column c + 8
+        }
         l_run += __shfl_xor(l_run, 16, 64);
         l_run += __shfl_xor(l_run, 32, 64);
         if (!live) return;
@@ -245,12 +279,14 @@ struct Mx4Math {
 };
 
 // NH: kv heads of a workgroup (neighbours in memory: their rows share lines).  STREAM: every line is one workgroup's alone, and
-// is loaded with the non-temporal hint; otherwise plain loads leave the lines in the L2 for the next reader.
-template <int QDT, int PM, int D, int MODE, int NH, bool STREAM>
+// is loaded with the non-temporal hint; otherwise plain loads leave the lines in the L2 for the next reader.  FOLDED: see
+// Mx4Math::Probs.
+template <int QDT, int PM, int D, int MODE, int NH, bool STREAM, bool FOLDED>
 __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, const Mx4Scales x) {
     static_assert(PM == PM_TILE || PM == PM_ROW, "page numbers per tile of 16 tokens, or per row");
     static_assert(!STREAM || NH == 1, "two buffers of one kv head's rows");
     using T = Mx4Tile<D>;
+    using Math = Mx4Math<QDT, D, FOLDED>;
     constexpr int DB = D / 16;                 // column blocks of O^T, values of a V row per lane
     constexpr int KSTEPS = D / 32;             // MFMA steps of a K row
     constexpr int kTileHeads = 16;
@@ -272,7 +308,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     int* const s_next = reinterpret_cast<int*>(sm_l + nw * NH * 16);
 
     auto write_empty_rows = [&](const int b, const int head0, const int heads_here) {
-        Mx4Math<QDT, D>::write_empty_rows(p, b, head0, heads_here, lane);
+        Math::write_empty_rows(p, b, head0, heads_here, lane);
     };
 
     // One piece: tokens [c_start, min(c_limit, kv_len)) of sequence b for kv heads NH hgb .. NH hgb + NH - 1 and q-head tile ht;
@@ -284,12 +320,12 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     const int kvh = hgb * NH;
     const int head0 = kvh * p.group + ht * kTileHeads;                     // + h * group for kv head kvh + h
     const int heads_here = min(kTileHeads, p.group - ht * kTileHeads);
-    // Q^T: lane (h = c, a) holds q[h][(D/4) a + 8 ks .. + 7] (columns past the group repeat its last head, and are not stored)
+    // Q^T: lane (h = c, a) holds q[h][(D/4) a + 8 ks .. + 7] (head_of)
     uint4 qb[NH][KSTEPS];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
         const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb +
-                             (int64_t)(head0 + h * p.group + min(c, heads_here - 1)) * p.q_sh + (D / 4) * a;
+                             (int64_t)(head0 + h * p.group + Math::head_of(c, heads_here)) * p.q_sh + (D / 4) * a;
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) qb[h][ks] = *reinterpret_cast<const uint4*>(qp + 8 * ks);
     }
@@ -450,9 +486,8 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
         for (int db = 0; db < DB; ++db) acc[h][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    using Math = Mx4Math<QDT, D>;
     auto softmax = [&](int t, float (&sv)[8], int h, auto masked_tag) {
-        return Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, c_end - (c_start + t * kStep), masked_tag);
+        return Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, c, c_end - (c_start + t * kStep), masked_tag);
     };
 
     // ---- pipeline ----
@@ -505,7 +540,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
 #pragma unroll
                 for (int h = 0; h < NH; ++h) Math::scores(r[h], qb[h], sv[h]);
                 if (more) issue_k(tn, pb, r, BoolTag<false>());
-                uint4 pv[NH];
+                typename Math::Probs pv[NH];
 #pragma unroll
                 for (int h = 0; h < NH; ++h) pv[h] = softmax(t, sv[h], h, BoolTag<false>());
 #pragma unroll
@@ -534,7 +569,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
 #pragma unroll
     for (int h = 0; h < NH; ++h)
         Math::leave_part(acc[h], m_run[h], l_run[h], lds + (wave * NH + h) * kScratch, sm_m + (wave * NH + h) * 16, sm_l + (wave * NH + h) * 16,
-                         live, lane);
+                         heads_here, lane);
     __syncthreads();
     if (live) {
 #pragma unroll
@@ -561,14 +596,19 @@ int launch_mx4(const SplitParams& p_in, const Mx4Scales& x, hipStream_t stream) 
     p.wavefronts = kWaves;
     const size_t lds_bytes = (size_t)kWaves * p.hg_per_wg * (D * 64 + 2 * 16 * sizeof(float)) + 16;
     const bool tile = p.page_shift >= 0 && p.page_size % 16 == 0;
-#define FDK_MX4_LAUNCH(PMV, MODEV, NHV, STV)                                                                                           \
+#define FDK_MX4_LAUNCH_OF(PMV, MODEV, NHV, STV, FV)                                                                                           \
     do {                                                                                                                               \
         if (lds_bytes > 64 * 1024) {                                                                                                   \
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&splitkv_mx4_kernel<QDT, PMV, D, MODEV, NHV, STV>), \
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&splitkv_mx4_kernel<QDT, PMV, D, MODEV, NHV, STV, FV>), \
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes);                      \
             if (e != hipSuccess) return (int)e;                                                                                        \
         }                                                                                                                              \
-        hipLaunchKernelGGL((splitkv_mx4_kernel<QDT, PMV, D, MODEV, NHV, STV>), grid, dim3(64 * kWaves), lds_bytes, stream, p, x);      \
+        hipLaunchKernelGGL((splitkv_mx4_kernel<QDT, PMV, D, MODEV, NHV, STV, FV>), grid, dim3(64 * kWaves), lds_bytes, stream, p, x);      \
+    } while (0)
+#define FDK_MX4_LAUNCH(PMV, MODEV, NHV, STV)                               \
+    do {                                                                   \
+        if (p.group <= 8) FDK_MX4_LAUNCH_OF(PMV, MODEV, NHV, STV, true);   \
+        else FDK_MX4_LAUNCH_OF(PMV, MODEV, NHV, STV, false);               \
     } while (0)
 #define FDK_MX4_LAUNCH_NH(NHV, STV)                                 \
     do {                                                            \
@@ -602,6 +642,7 @@ int launch_mx4(const SplitParams& p_in, const Mx4Scales& x, hipStream_t stream) 
     }
 #undef FDK_MX4_LAUNCH_NH
 #undef FDK_MX4_LAUNCH
+#undef FDK_MX4_LAUNCH_OF
     return (int)hipGetLastError();
 }
 

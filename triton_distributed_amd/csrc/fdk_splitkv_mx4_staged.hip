@@ -25,11 +25,11 @@ namespace {
 
 constexpr int kMx4Place = 2 * (32 * 128 + 32 * 2 * 4);      // bytes of a step's rows and scales
 
-template <int QDT, int MODE>
+template <int QDT, int MODE, bool FOLDED>
 __global__ __launch_bounds__(512) void splitkv_mx4_staged_kernel(const SplitParams p, const Mx4Scales x) {
     constexpr int D = 128, NH = 2;             // values of a row, kv heads of a workgroup
     using T = Mx4Tile<D>;
-    using Math = Mx4Math<QDT, D>;
+    using Math = Mx4Math<QDT, D, FOLDED>;
     constexpr int KSTEPS = D / 32, DB = D / 16;
     constexpr int kTileHeads = 16;
     constexpr bool kOneSegment = false;        // (fdk_splitkv_mfma_work.h: no single-launch form, units mapped to XCDs)
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_staged_kernel(const SplitPara
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
         const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q) + (int64_t)b * p.q_sb +
-                             (int64_t)(head0 + h * p.group + min(c, heads_here - 1)) * p.q_sh + (D / 4) * a;
+                             (int64_t)(head0 + h * p.group + Math::head_of(c, heads_here)) * p.q_sh + (D / 4) * a;
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) qb[h][ks] = *reinterpret_cast<const uint4*>(qp + 8 * ks);
     }
@@ -227,8 +227,8 @@ __global__ __launch_bounds__(512) void splitkv_mx4_staged_kernel(const SplitPara
         for (int h = 0; h < NH; ++h) {
             float sv[8];
             Math::scores(r[h], qb[h], sv);
-            if (left >= kStep) Math::values(r[h], Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, left, BoolTag<false>()), acc[h]);
-            else Math::values(r[h], Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, left, BoolTag<true>()), acc[h]);
+            if (left >= kStep) Math::values(r[h], Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, c, left, BoolTag<false>()), acc[h]);
+            else Math::values(r[h], Math::softmax(sv, m_run[h], l_run[h], acc[h], p, inv_cap, a, c, left, BoolTag<true>()), acc[h]);
         }
     }
 
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_staged_kernel(const SplitPara
 #pragma unroll
     for (int h = 0; h < NH; ++h)
         Math::leave_part(acc[h], m_run[h], l_run[h], lds + (wave * NH + h) * kScratch, sm_m + (wave * NH + h) * 16, sm_l + (wave * NH + h) * 16,
-                         live, lane);
+                         heads_here, lane);
     __syncthreads();
     if (live) {
 #pragma unroll
@@ -265,7 +265,8 @@ int launch_staged(const SplitParams& p_in, const Mx4Scales& x, hipStream_t strea
     // the places of all wavefronts; the merge needs 16 fp32 rows per wavefront and head, and m and l
     constexpr int kLds = kWaves * 2 * kMx4Place;
     static_assert(kLds >= kWaves * 2 * (128 * 64 + 2 * 16 * (int)sizeof(float)) + 16, "the merge");
-    auto* kernel = p.balanced ? &splitkv_mx4_staged_kernel<QDT, WM_SHARES> : &splitkv_mx4_staged_kernel<QDT, WM_ONE>;
+    auto* kernel = p.group <= 8 ? (p.balanced ? &splitkv_mx4_staged_kernel<QDT, WM_SHARES, true> : &splitkv_mx4_staged_kernel<QDT, WM_ONE, true>)
+                                : (p.balanced ? &splitkv_mx4_staged_kernel<QDT, WM_SHARES, false> : &splitkv_mx4_staged_kernel<QDT, WM_ONE, false>);
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) return (int)e;
     hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), kLds, stream, p, x);
