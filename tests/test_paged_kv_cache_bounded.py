@@ -43,6 +43,53 @@ def test_positions_and_refusals_without_a_gpu():
     assert c.max_kv_len == 7 and c.next_positions(1).tolist() == [[6]] * 3
 
 
+def _evict_on_the_host(monkeypatch):
+    """Stand-ins for the operators: lengths as the eviction leaves them; what the append is given."""
+    import triton_distributed_amd as tda
+    given = []
+
+    def evict(k, v, table, lens, w, keep, recent, kv_lens_out=None, **kw):
+        if kv_lens_out is not None:
+            kv_lens_out.clamp_(max=keep)
+
+    def append(*args, positions=None, **kw):
+        given.append(positions)
+    monkeypatch.setattr(tda, "evict_kvcache", evict, raising=False)
+    monkeypatch.setattr(tda, "qk_norm_rope_update_kvcache", append, raising=False)
+    return given
+
+
+def test_positions_behind_the_rotary_tables_are_refused(monkeypatch):
+    """A cache at a budget sees more tokens than it holds: from the first that the tables have no row for, an append that
+    would take its position from the count is refused, on the host; one with positions of its own is not."""
+    given = _evict_on_the_host(monkeypatch)
+    c = _cache("cpu")
+    w, table = torch.zeros(2, 3, 2, 64), torch.zeros(1, 40, 64)
+    x = torch.zeros(3, 1, 8, 64, dtype=torch.bfloat16)
+    c.inc_offset(30)
+    c.evict(w, 20, 5)
+    for seen in range(31, 41):
+        c.inc_offset(1)
+        c.append(0, x, None, None, table, table)
+        assert given[-1].tolist() == [[seen - 1]] * 3
+        if seen == 35:
+            c.evict(w, 20, 5)
+    assert c.max_kv_len == 25 < 40
+    c.inc_offset(1)
+    n = len(given)
+    for cos, sin in ((table, table), (table.expand(3, 40, 64), table[0]), (torch.zeros(50, 64), table)):
+        with pytest.raises(ValueError, match="positions"):
+            c.append(0, x, None, None, cos, sin)
+    assert len(given) == n
+    c.append(0, x, None, None, table, table, positions=torch.zeros(3, 1, dtype=torch.int32))
+    c.append(0, x, None, None, torch.zeros(41, 64), torch.zeros(41, 64))
+    assert len(given) == n + 2 and given[-1].tolist() == [[40]] * 3
+    c.reset()
+    c.inc_offset(2)
+    c.append(0, x, None, None, table[:, :1], table[:, :1])                  # (as ever without an eviction: places in the cache)
+    assert given[-1] is None and c.next_positions(1).tolist() == [[1]] * 3
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float4_e2m1fn_x2, torch.bfloat16])
 def test_a_serving_loop_at_a_budget(cuda_device, dtype):

@@ -19,7 +19,8 @@ Differences, all additions:
   * ``append`` / ``decode`` run the two operators of this package on one layer's view;
   * ``accumulate`` / ``evict`` keep the cache at a budget: attention weights per cached token, and the eviction of the
     tokens with the least of them from all layers.  From then on ``append`` takes the tokens' positions from a count of
-    the tokens seen (``next_positions``), not from their places in the cache.
+    the tokens seen (``next_positions``), not from their places in the cache; the cos / sin tables then need a row for every
+    token that a sequence will ever see, not for ``max_length`` of them.
 
 The class itself allocates with torch and launches nothing; it works on any torch device (the operators do not).
 """
@@ -123,6 +124,7 @@ class PagedKVCache:
         self.kv_lens = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
         self._host_len = 0
         self._seen = None               # [B] int32: tokens each sequence has seen, once some of them were evicted
+        self._host_seen = 0             # the same count on the host
 
     # ---- the reference's interface -----------------------------------------------------------------------------
     def inc_offset(self, seq_len: int) -> None:
@@ -134,6 +136,7 @@ class PagedKVCache:
         if self._seen is not None:
             self._seen += seq_len
         self._host_len += seq_len
+        self._host_seen += seq_len
 
     def get_layer_kv_cache(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
         """``(key_cache, value_cache, block_table [B, max_blocks_per_seq], kv_lens [B])`` of one layer
@@ -154,7 +157,7 @@ class PagedKVCache:
     def reset(self) -> None:
         """Forget all tokens; the pages keep their contents and their owners."""
         self.kv_lens.zero_()
-        self._host_len = 0
+        self._host_len = self._host_seen = 0
         self._seen = None
 
     def layer_scales(self, layer_idx: int):
@@ -169,13 +172,18 @@ class PagedKVCache:
                q_norm_rope: Optional[torch.Tensor] = None, stream=None, **kwargs) -> torch.Tensor:
         """Norm + rotary + append of ``qkv [B, T, Hq + 2 Hkv, D]`` into one layer, after ``inc_offset(T)``.
         ``positions`` / ``rope_sections`` / ``rope_interleaved`` as in ``qk_norm_rope_update_kvcache``; after an eviction
-        ``positions`` defaults to ``next_positions(T)``.  Returns the normalised, rotated query ``[B, T, Hq, D]``."""
+        ``positions`` defaults to ``next_positions(T)``, which the tables must have rows for.  Returns the normalised, rotated
+        query ``[B, T, Hq, D]``."""
         from . import qk_norm_rope_update_kvcache
         if qkv.shape[1] > self._host_len:
             raise ValueError("call inc_offset(T) before append: kv_lens must count the new tokens")
         k, v, table, lens = self.get_layer_kv_cache(layer_idx)
         ks, vs = self.layer_scales(layer_idx)
         if self._seen is not None and kwargs.get("positions") is None:
+            # (the operator turns a position behind the tables' end by their last row)
+            if self._host_seen > min(cos_cache.shape[-2], sin_cache.shape[-2]):
+                raise ValueError(f"the cos / sin tables have {cos_cache.shape[-2]} positions, the sequences have seen {self._host_seen} "
+                                 "tokens: longer tables, or positions")
             with self._on(stream):
                 kwargs["positions"] = self.next_positions(qkv.shape[1])
         return qk_norm_rope_update_kvcache(qkv, k, v, table, lens, q_rms_weight, k_rms_weight, cos_cache, sin_cache,
