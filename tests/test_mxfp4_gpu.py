@@ -289,3 +289,29 @@ def test_scales_of_a_head_past_32_bit_offsets(cuda_device, d, page):
         got[-1] += [kk, vv, s, t]
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+def test_conversion_results_belong_to_the_stream_they_are_written_on(cuda_device):
+    """A result that is dropped while its kernel still has to run goes back to that stream's pool: the next tensor of the
+    current stream is another one, and keeps what is written to it."""
+    import triton_distributed_amd as tda
+    dev, side = cuda_device, torch.cuda.Stream()
+    x = torch.randn(4096, 8192, device=dev, dtype=torch.bfloat16)
+    codes, scales = tda.mxfp4_quantize(x)
+    torch.cuda.synchronize()
+    for convert in (lambda: tda.mxfp4_quantize(x, stream=side), lambda: (tda.mxfp4_dequantize(codes, scales, stream=side),)):
+        torch.cuda.empty_cache()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(int(2e7))
+        made = convert()
+        at = [t.data_ptr() for t in made]
+        shapes = [(t.shape, t.dtype) for t in made]
+        del made
+        mine = [torch.full(s, 5, dtype=t, device=dev) for s, t in shapes]
+        torch.cuda.synchronize()
+        assert not set(at) & {t.data_ptr() for t in mine}
+        assert all((t == 5).all() for t in mine)
+    c, s = tda.mxfp4_quantize(x, stream=side)
+    y = tda.mxfp4_dequantize(c, s, stream=side)
+    side.synchronize()
+    assert torch.equal(c, codes) and torch.equal(s, scales) and torch.equal(y, tda.mxfp4_dequantize(codes, scales))

@@ -1025,6 +1025,15 @@ def _mxfp4_convert(fn, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tenso
         _MXFP4_TEMPLATES[key] = bytes(a)
 
 
+def _mxfp4_empty(like: torch.Tensor, last: int, dtype: torch.dtype, stream) -> torch.Tensor:
+    """A result ``[..., last]`` beside ``like``, from the pool of the stream that the conversion runs on: a result that is
+    dropped while it runs must go back there."""
+    if stream is None or not like.is_cuda:
+        return torch.empty(like.shape[:-1] + (last,), dtype=dtype, device=like.device)
+    with _on_stream(like.device, _stream_handle(stream)):
+        return torch.empty(like.shape[:-1] + (last,), dtype=dtype, device=like.device)
+
+
 def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *,
                    stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """bf16 / fp16 rows ``[..., D]`` as MXFP4: ``(codes [..., D/2] uint8, scales [..., D/32] uint8)`` - what the append
@@ -1034,9 +1043,9 @@ def mxfp4_quantize(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales
     and [2^-126, 2^13] for fp16; codes are rounded to nearest, ties to even, and saturate at 6 scales.  A block with an
     infinity or a NaN in it reads as NaN (scale byte 255)."""
     if codes is None:
-        codes = torch.empty(x.shape[:-1] + (x.shape[-1] // 2,), dtype=torch.uint8, device=x.device)
+        codes = _mxfp4_empty(x, x.shape[-1] // 2, torch.uint8, stream)
     if scales is None:
-        scales = torch.empty(x.shape[:-1] + (x.shape[-1] // MXFP4_BLOCK,), dtype=torch.uint8, device=x.device)
+        scales = _mxfp4_empty(x, x.shape[-1] // MXFP4_BLOCK, torch.uint8, stream)
     _mxfp4_convert(_LIB.fdk_mx_quantize, x, codes, scales, stream)
     return codes, scales
 
@@ -1045,6 +1054,6 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dty
                      out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """The values MXFP4 rows stand for, ``code * 2^(scale byte - 127)``, as bf16 / fp16 ``[..., D]``."""
     if out is None:
-        out = torch.empty(codes.shape[:-1] + (codes.shape[-1] * 2,), dtype=dtype, device=codes.device)
+        out = _mxfp4_empty(codes, codes.shape[-1] * 2, dtype, stream)
     _mxfp4_convert(_LIB.fdk_mx_dequantize, out, codes, scales, stream)
     return out
