@@ -392,7 +392,7 @@ typedef struct fdk_kv_evict_args {
     int32_t kv_dtype;     /* FDK_BF16 | FDK_FP16 | FDK_FP8_E4M3 | FDK_MXFP4 */
     int32_t reserved0;
     void* k_cache;        /* [num_pages, P, Hkv, D], rows of a multiple of 16 bytes */
-    void* v_cache;        /* [num_pages, P, Hkv, Dv] */
+    void* v_cache;        /* [num_pages, P, Hkv, Dv]; may be a part of the K rows (same strides), which then move once */
     int64_t k_stride_page, k_stride_tok, k_stride_head;
     int64_t v_stride_page, v_stride_tok, v_stride_head;
     uint8_t* k_block_scale; /* MXFP4 caches: the scales move with the rows; byte strides */

@@ -347,3 +347,31 @@ def test_rows_of_pages_outside_the_pool_are_left_out(cuda_device, kind, bad):
     assert lens.tolist() == [32] * 3 and kept[0, 0].tolist() == list(range(32, 64))
     for t, w in zip(got, want):
         assert torch.equal(t.cpu(), w)
+
+
+@pytest.mark.parametrize("dk,dv,first,hkv", [(576, 512, 0, 1), (576, 512, 64, 1), (128, 128, 0, 4), (64, 128, 0, 2)])
+@pytest.mark.parametrize("lens,keep", [([700, 90, 300], 200), ([5000], 3000)])
+def test_v_rows_that_are_a_part_of_the_k_rows(cuda_device, dk, dv, first, hkv, lens, keep):
+    """Latent attention holds V inside K (and, the other way round, K inside V): every row moves once, whole."""
+    import triton_distributed_amd as tda
+    dev, page, d = cuda_device, 16, max(dk, dv)
+    c, table, _, _ = _cache("16bit", lens, page, hkv, d, torch.bfloat16, dk + first)
+    pool = c["k"].to(dev)
+    k, v = (pool, pool[..., first:first + dv]) if dk >= dv else (pool[..., first:first + dk], pool)
+    w = (torch.rand(len(lens), hkv, max(lens), generator=torch.Generator().manual_seed(4)) ** 4 * 64).round() / 64
+    n = torch.tensor(lens, dtype=torch.int32, device=dev)
+    new, kept, wo = tda.evict_kvcache(k, v, table.to(dev), n, w.to(dev), keep, 50)
+    (want,), want_new, want_kept, want_w = okv.evict([c["k"]], table, lens, w, keep, 50)
+    assert torch.equal(new.cpu(), want_new) and torch.equal(kept.cpu(), want_kept) and torch.equal(wo.cpu(), want_w)
+    assert torch.equal(pool.cpu(), want)
+
+
+def test_mxfp4_rows_and_scales_that_are_v_and_k_at_once(cuda_device):
+    import triton_distributed_amd as tda
+    dev, lens = cuda_device, [400, 77]
+    c, table, _, _ = _cache("mxfp4", lens, 16, 2, 128, torch.bfloat16, 6)
+    rows, scales = c["k"].to(dev), c["ks"].to(dev)
+    w = torch.rand(2, 2, 400, generator=torch.Generator().manual_seed(4))
+    tda.evict_kvcache(rows, rows, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), w.to(dev), 60, 5, k_scale=scales, v_scale=scales)
+    (want_rows, want_scales), _, _, _ = okv.evict([c["k"], c["ks"]], table, lens, w, 60, 5)
+    assert torch.equal(rows.cpu(), want_rows) and torch.equal(scales.cpu(), want_scales)

@@ -79,6 +79,17 @@ def test_evict_refusals(kw, code):
     assert _lib.load().fdk_kv_evict(C.byref(_evict_args(**kw)), None) == code, _lib.load().fdk_last_error()
 
 
+@pytest.mark.parametrize("kw,code", [
+    (dict(v_cache=0x10000), 0), (dict(v_cache=0x10000, v_head_dim=64), 0), (dict(v_cache=0x10080, v_head_dim=64), 0),
+    (dict(k_cache=0x10080, v_cache=0x10000, head_dim=64), 0), (dict(v_cache=0x10100), 0), (dict(v_cache=0x10080), _lib.FDK_ESHAPE),
+    (dict(v_cache=0x0FF80), _lib.FDK_ESHAPE), (dict(v_cache=0x0FF00), 0),
+    (dict(v_cache=0x10080, batch=1, num_kv_heads=1, v_stride_head=999), _lib.FDK_ESHAPE),
+])
+def test_rows_that_share_memory(kw, code):
+    """V rows that are a part of the K rows, or the other way round, are one thing to move; rows of which parts overlap are refused."""
+    assert _lib.load().fdk_kv_evict(C.byref(_evict_args(**kw)), None) == code, _lib.load().fdk_last_error()
+
+
 def test_workspace_of_long_rows():
     """One plan entry a row; rows that few workgroups would have to themselves need room for counts and weights."""
     lib = _lib.load()

@@ -1110,6 +1110,20 @@ size_t fdk_kv_evict_workspace_bytes(const fdk_kv_evict_args* a) {
     return fdk::evict_workspace_bytes(a->batch, a->num_kv_heads, evict_max_tokens(a), a->keep, cus);
 }
 
+// Rows of `a` and `b` that share memory token by token (latent attention: the V rows are a part of the K rows) are moved once, by
+// the tensor whose rows hold the other's; moved twice, each would overwrite what the other still has to read.  False: parts of
+// rows overlap, and neither holds the other.
+static bool share_rows(fdk::EvictRows& a, fdk::EvictRows& b, int num_kv_heads, int page_size, int num_pages) {
+    if ((num_pages > 1 && a.sp != b.sp) || (page_size > 1 && a.st != b.st) || (num_kv_heads > 1 && a.sh != b.sh)) return true;
+    const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(b.pool) - reinterpret_cast<uintptr_t>(a.pool));
+    const int64_t na = (int64_t)a.cols * a.bytes, nb = (int64_t)b.cols * b.bytes;
+    if (at >= na || at <= -nb) return true;
+    if (at >= 0 && at + nb <= na) b.cols = 0;
+    else if (at <= 0 && at + nb >= na) a.cols = 0;
+    else return false;
+    return true;
+}
+
 int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     g_err[0] = 0;
     if (!caller_args) return fail(FDK_ENULL, "args is null");
@@ -1142,6 +1156,20 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
         if (!rc) rc = check_scale_strides(nullptr, a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head, dv, a->num_kv_heads, a->page_size);
         if (rc) return rc;
     }
+    fdk::EvictParams p;
+    memset(&p, 0, sizeof(p));
+    p.num_tensors = mx ? 4 : 2;
+    p.rows[0] = fdk::EvictRows{static_cast<char*>(a->k_cache), a->k_stride_page * es, a->k_stride_tok * es, a->k_stride_head * es, kb / 16, 16};
+    p.rows[1] = fdk::EvictRows{static_cast<char*>(a->v_cache), a->v_stride_page * es, a->v_stride_tok * es, a->v_stride_head * es, vb / 16, 16};
+    if (mx) {
+        p.rows[2] = fdk::EvictRows{reinterpret_cast<char*>(a->k_block_scale), a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head,
+                                   a->head_dim / fdk::kMxBlock, 1};
+        p.rows[3] = fdk::EvictRows{reinterpret_cast<char*>(a->v_block_scale), a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head,
+                                   dv / fdk::kMxBlock, 1};
+    }
+    if (!share_rows(p.rows[0], p.rows[1], a->num_kv_heads, a->page_size, a->num_pages) ||
+        !share_rows(p.rows[2], p.rows[3], a->num_kv_heads, a->page_size, a->num_pages))
+        return fail(FDK_ESHAPE, "parts of k_cache and v_cache rows overlap");
     if (!a->weights || !a->weights_out || !a->kept || !a->kv_lens_out)
         return fail(FDK_ENULL, "weights / weights_out / kept / kv_lens_out must be non-null");
     if ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out) | reinterpret_cast<uintptr_t>(a->kept) |
@@ -1157,17 +1185,6 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     if (!a->workspace || a->workspace_bytes < need) return fail(FDK_EWORKSPACE, "workspace has %zu bytes; %zu needed", a->workspace ? a->workspace_bytes : 0, need);
     if (!aligned16(a->workspace)) return fail(FDK_EALIGN, "workspace must be 16-byte aligned");
     if (a->flags & FDK_FLAG_DRY_RUN) return FDK_OK;
-    fdk::EvictParams p;
-    memset(&p, 0, sizeof(p));
-    p.num_tensors = mx ? 4 : 2;
-    p.rows[0] = fdk::EvictRows{static_cast<char*>(a->k_cache), a->k_stride_page * es, a->k_stride_tok * es, a->k_stride_head * es, kb / 16, 16};
-    p.rows[1] = fdk::EvictRows{static_cast<char*>(a->v_cache), a->v_stride_page * es, a->v_stride_tok * es, a->v_stride_head * es, vb / 16, 16};
-    if (mx) {
-        p.rows[2] = fdk::EvictRows{reinterpret_cast<char*>(a->k_block_scale), a->kbs_stride_page, a->kbs_stride_tok, a->kbs_stride_head,
-                                   a->head_dim / fdk::kMxBlock, 1};
-        p.rows[3] = fdk::EvictRows{reinterpret_cast<char*>(a->v_block_scale), a->vbs_stride_page, a->vbs_stride_tok, a->vbs_stride_head,
-                                   dv / fdk::kMxBlock, 1};
-    }
     p.block_table = a->block_table; p.kv_lens = a->kv_lens; p.weights = a->weights; p.weights_out = a->weights_out;
     p.kept = a->kept; p.plan = static_cast<int32_t*>(a->workspace); p.kv_lens_out = a->kv_lens_out;
     p.tbl_sb = a->table_stride_b; p.w_sb = a->weights_stride_b; p.w_sh = a->weights_stride_h;

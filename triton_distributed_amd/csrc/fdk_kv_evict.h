@@ -29,7 +29,8 @@ struct AttnWeightsParams {
     float scale_log2, sm_scale, soft_cap;
 };
 
-// rows of one tensor of the cache: `cols` pieces of 16 bytes (or single bytes: the block scales)
+// rows of one tensor of the cache: `cols` pieces of 16 bytes (or single bytes: the block scales); none where another tensor's
+// rows hold them
 struct EvictRows {
     char* pool;
     int64_t sp, st, sh;                      // byte strides of the page, token and head axes

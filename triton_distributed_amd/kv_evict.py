@@ -139,7 +139,7 @@ def evict_kvcache(key_cache: torch.Tensor, value_cache: torch.Tensor, block_tabl
 
     key_cache, value_cache  [num_pages, P, Hkv, D] (any row length that is a multiple of 32 values; 16-bit, fp8), or MXFP4
                  codes with their block scales k_scale / v_scale, which move along; the scales of an fp8 cache do not depend on
-                 the tokens and are not asked for
+                 the tokens and are not asked for.  value_cache may be a view of key_cache's rows (latent attention)
     block_table  [B, max_pages] int32, kv_lens [B] int32, weights [B, Hkv, S] fp32 with S covering every length
     keep, recent 1 <= keep <= S, 0 <= recent <= keep; a sequence of at most ``keep`` tokens stays as it is
 
