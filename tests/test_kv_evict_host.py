@@ -90,6 +90,24 @@ def test_rows_that_share_memory(kw, code):
     assert _lib.load().fdk_kv_evict(C.byref(_evict_args(**kw)), None) == code, _lib.load().fdk_last_error()
 
 
+def test_weights_rows_that_share_elements_are_refused():
+    """Every layout of three sequences x four heads with strides up to 60 elements, rows of 5: against the elements themselves."""
+    lib = _lib.load()
+    for sb in range(5, 60):
+        for sh in range(5, 60):
+            at = [b * sb + h * sh + i for b in range(3) for h in range(4) for i in range(5)]
+            want = 0 if len(set(at)) == len(at) else _lib.FDK_ESHAPE
+            a = _weights_args(batch=3, num_kv_heads=4, num_q_heads=4, weights_len=5, weights_stride_b=sb, weights_stride_h=sh, lse_stride_b=4)
+            assert lib.fdk_accumulate_weights(C.byref(a), None) == want, (sb, sh)
+            e = _evict_args(batch=3, num_kv_heads=4, weights_len=5, keep=3, recent=1, weights_out_stride_b=sb, weights_out_stride_h=sh)
+            assert lib.fdk_kv_evict(C.byref(e), None) == want, (sb, sh)
+    # large strides, one axis alone
+    assert lib.fdk_accumulate_weights(C.byref(_weights_args(weights_stride_b=4096, weights_stride_h=4096 * 31)), None) == _lib.FDK_ESHAPE
+    assert lib.fdk_accumulate_weights(C.byref(_weights_args(weights_stride_b=4096, weights_stride_h=4096 * 32)), None) == 0
+    assert lib.fdk_accumulate_weights(C.byref(_weights_args(batch=1, weights_stride_b=0)), None) == 0
+    assert lib.fdk_accumulate_weights(C.byref(_weights_args(weights_stride_b=1 << 61, weights_stride_h=1 << 60)), None) == _lib.FDK_ESHAPE
+
+
 def test_workspace_of_long_rows():
     """One plan entry a row; rows that few workgroups would have to themselves need room for counts and weights."""
     lib = _lib.load()

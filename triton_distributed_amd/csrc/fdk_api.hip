@@ -1037,6 +1037,25 @@ static int check_rows(const char* what, const void* cache, int64_t sp, int64_t s
     return FDK_OK;
 }
 
+// Whether any two of batch x heads rows of `length` elements, sb and sh apart, share an element.  (128 bits: the strides are the
+// caller's)
+static bool rows_overlap(int batch, int heads, __int128 sb, __int128 sh, int64_t length) {
+    if (batch == 1) return heads > 1 && sh < length;
+    if (heads == 1) return sb < length;
+    if (sb < length || sh < length) return true;
+    if (sb >= (heads - 1) * sh + length || sh >= (batch - 1) * sb + length) return false;         // one axis inside the other
+    // two rows that are i and -j apart on the two axes: every multiple of the larger stride and the multiples of the other next to it
+    const __int128 outer = sb > sh ? sb : sh, inner = sb > sh ? sh : sb;
+    const int n_outer = sb > sh ? batch : heads, n_inner = sb > sh ? heads : batch;
+    for (int i = 1; i < n_outer; ++i) {
+        const __int128 j = i * outer / inner;
+        if (j < n_inner && i * outer - j * inner < length) return true;
+        if (j + 1 < n_inner && (j + 1) * inner - i * outer < length) return true;
+        if (j >= n_inner) break;                       // (and so do all further multiples)
+    }
+    return false;
+}
+
 int fdk_accumulate_weights(const fdk_attn_weights_args* caller_args, void* hip_stream) {
     g_err[0] = 0;
     if (!caller_args) return fail(FDK_ENULL, "args is null");
@@ -1069,7 +1088,7 @@ int fdk_accumulate_weights(const fdk_attn_weights_args* caller_args, void* hip_s
         return fail(FDK_EALIGN, "lse / weights / k_scale must be 4-byte aligned");
     if (a->lse_stride_b < a->num_q_heads) return fail(FDK_ESHAPE, "lse_stride_b %lld < Hq", (long long)a->lse_stride_b);
     // (every weight is one wavefront's: rows must not overlap)
-    if ((a->num_kv_heads > 1 && a->weights_stride_h < a->weights_len) || (a->batch > 1 && a->weights_stride_b < a->weights_len))
+    if (rows_overlap(a->batch, a->num_kv_heads, a->weights_stride_b, a->weights_stride_h, a->weights_len))
         return fail(FDK_ESHAPE, "weights rows overlap");
     if (mx) {
         if (!a->k_block_scale) return fail(FDK_ENULL, "k_block_scale is required for an mxfp4 cache");
@@ -1175,7 +1194,7 @@ int fdk_kv_evict(const fdk_kv_evict_args* caller_args, void* hip_stream) {
     if ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out) | reinterpret_cast<uintptr_t>(a->kept) |
          reinterpret_cast<uintptr_t>(a->kv_lens_out)) & 3u)
         return fail(FDK_EALIGN, "weights / weights_out / kept / kv_lens_out must be 4-byte aligned");
-    if ((a->num_kv_heads > 1 && a->weights_out_stride_h < a->weights_len) || (a->batch > 1 && a->weights_out_stride_b < a->weights_len))
+    if (rows_overlap(a->batch, a->num_kv_heads, a->weights_out_stride_b, a->weights_out_stride_h, a->weights_len))
         return fail(FDK_ESHAPE, "weights_out rows overlap");
     if (a->weights_stride_b < 0 || a->weights_stride_h < 0) return fail(FDK_ESHAPE, "negative weights stride");
     if (a->weights == a->weights_out &&
