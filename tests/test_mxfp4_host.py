@@ -130,6 +130,26 @@ def test_conversion_refusals(kw, code):
         assert fn(C.byref(_conv(**kw)), None) == code
 
 
+@pytest.mark.parametrize("name,row", [("codes_stride", 64), ("scales_stride", 4), ("x_stride", 128)])
+@pytest.mark.parametrize("axis", [0, 1, 2])
+def test_conversion_results_whose_rows_overlap(name, row, axis):
+    """A row that is read may stand for many (stride 0); rows that are written have memory of their own."""
+    lib = _lib.load()
+    strides = dict(x_stride=[128] * 3, codes_stride=[64] * 3, scales_stride=[4] * 3)
+    n = [1, 1, 1]
+    n[axis] = 7
+    for stride, apart in ((0, False), (row // 2, False), (row, True)):
+        st = {k: list(v) for k, v in strides.items()}
+        st[name][axis] = stride
+        a = _conv(n=(C.c_int32 * 3)(*n), **{k: (C.c_int64 * 3)(*v) for k, v in st.items()})
+        writes = lib.fdk_mx_dequantize if name == "x_stride" else lib.fdk_mx_quantize
+        reads = lib.fdk_mx_quantize if name == "x_stride" else lib.fdk_mx_dequantize
+        assert reads(C.byref(a), None) == 0
+        assert writes(C.byref(a), None) == (0 if apart else _lib.FDK_ESHAPE)
+        a.n[axis] = 1                                               # (one row: its stride is not used)
+        assert writes(C.byref(a), None) == 0
+
+
 def test_python_refusals():
     x = torch.zeros(4, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="live on the GPU"):

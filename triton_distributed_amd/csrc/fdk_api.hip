@@ -870,6 +870,10 @@ static int mxfp4_convert(const fdk_mxfp4_args* caller_args, bool quantize, void*
         if (a->x_stride[i] < 0 || a->codes_stride[i] < 0 || a->scales_stride[i] < 0) return fail(FDK_ESHAPE, "negative stride");
         if (a->n[i] > 1 && (a->x_stride[i] % 8 || a->codes_stride[i] % 4))
             return fail(FDK_EALIGN, "rows of x must be 16-byte aligned, rows of codes 4-byte aligned");
+        // (what is read may repeat a row; two threads must not write the same one)
+        if (a->n[i] > 1 && (quantize ? a->codes_stride[i] < a->num_values / 2 || a->scales_stride[i] < a->num_values / fdk::kMxBlock
+                                     : a->x_stride[i] < a->num_values))
+            return fail(FDK_ESHAPE, "rows of the result overlap");
     }
     if (!aligned16(a->x) || (reinterpret_cast<uintptr_t>(a->codes) & 3u))
         return fail(FDK_EALIGN, "x must be 16-byte aligned, codes 4-byte aligned");
