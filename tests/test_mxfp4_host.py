@@ -259,3 +259,21 @@ def test_append_blocks():
     a, x = _append_args(dict(positions=None, num_axes=0, kv_dtype=_lib.FDK_BF16, k_stride_head=128, v_stride_head=128,
                              k_block_scale=None))
     assert lib.fdk_kv_append_axes(C.byref(x), None) == 0
+
+
+def test_entry_points_without_block_scales_say_so():
+    """The drop-ins for the reference's functions, and the layer over them, cannot be given the scales of a 4-bit cache."""
+    from triton_distributed_amd.sp_flash_decode_layer import SpGQAFlashDecodeAttention
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    table, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    layer = SpGQAFlashDecodeAttention(0, 0, 1, 1, 4, 2, 128, 128)
+    for cache in (torch.zeros(2, 16, 2, 64, dtype=torch.uint8), torch.zeros(2, 16, 2, 64, dtype=torch.uint8).view(torch.float4_e2m1fn_x2)):
+        for fn in (tda.gqa_fwd_batch_decode, tda.gqa_fwd_batch_decode_intra_rank, tda.gqa_fwd_batch_decode_persistent):
+            with pytest.raises(ValueError, match=f"{fn.__name__} takes no block scales"):
+                fn(q, cache, cache, None, [1], n, table, 0.1)
+            with pytest.raises(ValueError, match="flash_decode"):
+                getattr(tda, fn.__name__ + "_aot")(None, q, cache, cache, None, [1], n, table, 0.1)
+        with pytest.raises(ValueError, match="flash_decode_bsnh takes no block scales"):
+            tda.flash_decode_bsnh(q[:, None], cache, cache, table, n)
+        with pytest.raises(ValueError, match="takes no block scales"):
+            layer(q, cache, cache, n[None], table)

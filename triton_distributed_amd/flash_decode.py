@@ -609,6 +609,13 @@ def _drop_in_bounds(q, kv_lens, fb):
     return fb, lo, hi
 
 
+def _no_block_scales(entry: str, k_cache) -> None:
+    """The entry points with the reference's signatures have no place for the block scales of an MXFP4 cache."""
+    if k_cache.dtype in _MXFP4_CODES:
+        raise ValueError(f"{entry} takes no block scales, and so no MXFP4 cache: call flash_decode or prepare_decode "
+                         "(packed_out= for the packed result)")
+
+
 def gqa_fwd_batch_decode_intra_rank(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table, scale,
                                     soft_cap=0.0, output_split=None, output_combine=None, kv_split=-1,
                                     stream=None, length_feedback: Optional[LengthFeedback] = None):
@@ -619,6 +626,7 @@ def gqa_fwd_batch_decode_intra_rank(q, k_cache, v_cache, workspace, q_lens, kv_l
     ``length_feedback`` (not in the reference): a ``LengthFeedback`` that the caller keeps for this batch; the call
     plans with the bounds the previous call left there and leaves its own (see ``LengthFeedback``).  Without it the
     call knows nothing about the lengths and every call plans alike."""
+    _no_block_scales("gqa_fwd_batch_decode_intra_rank", k_cache)
     batch, q_heads = q.shape[:2]
     d = v_cache.shape[-1]
     if output_combine is None:
@@ -639,6 +647,7 @@ def gqa_fwd_batch_decode(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_
                          output_split=None, output_combine=None, kv_split=-1, stream=None,
                          length_feedback: Optional[LengthFeedback] = None):
     """Drop-in for the reference function of the same name (flash_decode.py:763-844): ``[B, Hq, D]``."""
+    _no_block_scales("gqa_fwd_batch_decode", k_cache)
     if q.is_cuda:
         stream = _stream_handle(stream)
     fb, lo, hi = _drop_in_bounds(q, kv_lens, length_feedback)
@@ -675,6 +684,7 @@ def gqa_fwd_batch_decode_persistent(q, k_cache, v_cache, workspace, q_lens, kv_l
     (common_ops.py:57-81), whereas the queue's counters must be zero on entry, so the library always uses counters
     of its own (per stream, left at zero by every call).  The result is in q's dtype (the reference allocates
     float16 whatever q is)."""
+    _no_block_scales("gqa_fwd_batch_decode_persistent", k_cache)
     splits, planned = _reference_kv_split(32 if kv_split == -1 else kv_split, q, k_cache, v_cache, block_table, kv_lens,
                                           scale, soft_cap)
     if q.is_cuda:
@@ -775,6 +785,7 @@ def flash_decode_bsnh(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
 
     query / output ``[B, 1, Hq, D]`` (one new token per sequence, :274), caches ``[num_pages, P, Hkv, D]``,
     ``sm_scale`` defaults to ``D ** -0.5`` (:275-276).  ``soft_cap`` is honoured (the builder zeroes it, :277)."""
+    _no_block_scales("flash_decode_bsnh", key_cache)
     if query.dim() != 4 or query.shape[1] != 1:
         raise ValueError("query must be [B, 1, Hq, D]: flash decoding takes one query token per sequence")
     batch, _, q_heads, d = query.shape
