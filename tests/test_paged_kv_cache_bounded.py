@@ -90,6 +90,42 @@ def test_positions_behind_the_rotary_tables_are_refused(monkeypatch):
     assert given[-1] is None and c.next_positions(1).tolist() == [[1]] * 3
 
 
+def test_an_eviction_is_not_captured(monkeypatch):
+    """A replay would shorten the sequences once more and count the tokens seen from the shortened lengths, while the host
+    goes on from what it knew at the capture."""
+    import sys
+    _evict_on_the_host(monkeypatch)
+    c = _cache("cpu")
+    w = torch.zeros(2, 3, 2, 64)
+    c.inc_offset(30)
+    monkeypatch.setattr(sys.modules["triton_distributed_amd.flash_decode"], "_capturing", lambda: True)
+    with pytest.raises(ValueError, match="capture"):
+        c.evict(w, 20, 5)
+    assert c.max_kv_len == 30 and c.kv_lens.tolist() == [30] * 3 and c.next_positions(1).tolist() == [[29]] * 3
+    assert c.evict(w, 30, 5) is None
+    monkeypatch.undo()
+    _evict_on_the_host(monkeypatch)
+    assert tuple(c.evict(w, 20, 5).shape) == (2, 3, 2, 20) and c.max_kv_len == 20
+
+
+@pytest.mark.gpu
+def test_an_eviction_under_capture_leaves_the_cache_as_it_was(cuda_device):
+    c = _cache(cuda_device)
+    c.inc_offset(30)
+    w = torch.rand(2, 3, 2, 64, device=cuda_device)
+    x = torch.zeros(1, device=cuda_device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(ValueError, match="capture"):
+            c.evict(w, 20, 5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert c.max_kv_len == 30 and c.kv_lens.tolist() == [30] * 3 and float(x) == 1
+    assert tuple(c.evict(w, 20, 5).shape) == (2, 3, 2, 20) and c.kv_lens.tolist() == [20] * 3
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float4_e2m1fn_x2, torch.bfloat16])
 def test_a_serving_loop_at_a_budget(cuda_device, dtype):

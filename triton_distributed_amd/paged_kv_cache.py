@@ -213,13 +213,17 @@ class PagedKVCache:
 
     def evict(self, weights: torch.Tensor, keep: int, recent: int, stream=None) -> Optional[torch.Tensor]:
         """Bring every layer back to at most ``keep`` tokens by its weights ``[num_layers, B, Hkv, S]``, which move along
-        (see ``evict_kvcache``).  Returns ``kept [num_layers, B, Hkv, keep]``, or None if nothing had to go."""
+        (see ``evict_kvcache``).  Returns ``kept [num_layers, B, Hkv, keep]``, or None if nothing had to go.  Not to be captured
+        into a graph: it changes the host's count of tokens, which a replay does not."""
         from . import evict_kvcache
         if weights.dim() != 4 or weights.shape[0] != self.num_layers or weights.shape[3] < self._host_len:
             raise ValueError(f"weights must be [{self.num_layers}, B, Hkv, S] with S >= {self._host_len} tokens")
         if self._host_len <= keep:
             return None
         with self._on(stream):
+            from .flash_decode import _capturing
+            if _capturing():
+                raise ValueError("an eviction changes the host's count of tokens: not under graph capture (evict_kvcache can be captured)")
             kept = torch.empty((self.num_layers, self.batch_size, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
             seen = self.kv_lens.clone() if self._seen is None else self._seen
         scales = {} if not self.mxfp4 else dict(k_scale=self.k_block_scale, v_scale=self.v_block_scale)
