@@ -65,11 +65,6 @@ __device__ __forceinline__ uint32_t mx_scale_byte(float amax, int max_exp) {
 }
 template <int QDT> __device__ __forceinline__ constexpr int mx_max_exp() { return QDT == FDK_BF16 ? 125 : 13; }
 
-// one e2m1 code (four bits) of x / scale
-__device__ __forceinline__ uint32_t mx_code(float x, float scale) {
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x, x, scale, 0) & 15u;
-}
-
 #endif  // __HIPCC__
 
 }  // namespace fdk
