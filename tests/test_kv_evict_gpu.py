@@ -375,3 +375,17 @@ def test_mxfp4_rows_and_scales_that_are_v_and_k_at_once(cuda_device):
     tda.evict_kvcache(rows, rows, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), w.to(dev), 60, 5, k_scale=scales, v_scale=scales)
     (want_rows, want_scales), _, _, _ = okv.evict([c["k"], c["ks"]], table, lens, w, 60, 5)
     assert torch.equal(rows.cpu(), want_rows) and torch.equal(scales.cpu(), want_scales)
+
+
+@pytest.mark.parametrize("b,hkv,length,keep,recent,d", [(1, 1, 4097, 4000, 100, 32), (1, 3, 16384, 16000, 0, 32), (2, 16, 12001, 300, 300, 32),
+                                                        (4, 64, 9000, 2000, 17, 32), (4, 64, 20000, 19000, 17, 32), (2, 40, 70000, 1000, 10, 32)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_long_rows_of_one_workgroup_each(cuda_device, b, hkv, length, keep, recent, d, in_place):
+    """Up to 16384 weights out of registers; longer rows, of which there are many, read in every pass."""
+    test_rows_spread_over_workgroups(cuda_device, b, hkv, length, keep, recent, d, in_place)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_segments_that_are_read_in_every_pass(cuda_device, in_place):
+    """Eight workgroups to a row, of more than 16384 weights each."""
+    test_rows_spread_over_workgroups(cuda_device, 1, 64, 140000, 700, 10, 32, in_place)

@@ -122,6 +122,18 @@ def test_workspace_of_long_rows():
     assert lib.fdk_kv_evict_workspace_bytes(None) == 0
 
 
+def test_workspace_says_which_rows_are_shared_out():
+    """Rows that one workgroup holds in registers, and rows of which there are enough for the compute units, stay one workgroup's."""
+    lib = _lib.load()
+
+    def shared(batch, length):
+        a = _evict_args(batch=batch, max_pages=length // 16 + 1, table_stride_b=length // 16 + 1, weights_len=length)
+        return lib.fdk_kv_evict_workspace_bytes(C.byref(a)) > batch * 8 * 16
+    assert [shared(1, n) for n in (4097, 8192, 16384, 16385, 65536, 1 << 20)] == [False, False, False, True, True, True]
+    assert [shared(b, 65536) for b in (8, 9, 16, 32, 200)] == [True, False, False, False, False]
+    assert [shared(1, n) for n in (64 * 65471, 64 * 65471 + 1)] == [True, False]              # (counts of 16 bits)
+
+
 def test_python_refusals():
     k = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
     table, n, w = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 2, 64)

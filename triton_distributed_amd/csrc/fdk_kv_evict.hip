@@ -522,15 +522,22 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const MoveParams m)
 
 }  // namespace
 
-// Segments of a row: two workgroups per compute unit where rows are few and long, none below 4096 weights to a segment.
+// Segments of a row (of its capacity: the lengths are on the device): as many as give two workgroups to a compute unit, of about
+// 4096 weights or more.  One workgroup does it in one launch instead of four, up to 16384 weights out of registers; more are for
+// longer rows, and for few of them: whole calls, a quarter kept, in us, one workgroup to a row against several (rows of 256 bytes)
+// 8 rows of 4097 / 8192 / 16384 tokens 25 / 28 / 42 against 32 / 32 / 42, 256 rows 72 / 134 / 257 against 113 / 195 / 385; (rows of
+// 128 bytes) 8 rows of 16400 / 65536 tokens 49 / 140 against 39 / 67, 64 rows (eight segments) 78 / 258 against 79 / 190, 128 rows
+// (four) 108 / 389 against 127 / 376, 256 rows (two) 177 / 653 against 229 / 890.
 int evict_segments(int batch, int hkv, int max_tokens, int num_cus) {
     int64_t s = 2 * (int64_t)num_cus / ((int64_t)batch * hkv);
+    if (max_tokens <= 16 * kSelectThreads || s < 8) return 1;
     const int64_t most = ((int64_t)max_tokens + 4095) / 4096;
     if (s > most) s = most;
     if (s > kMaxSegments) s = kMaxSegments;
-    // (16-bit counts)
-    const int64_t least = ((int64_t)max_tokens + 65535 - 64) / (65535 - 64);
-    return s < 2 || s < least ? 1 : (int)s;
+    // (16-bit counts; a segment is rounded up to a multiple of 64)
+    constexpr int64_t kLargest = 65535 - 64;
+    const int64_t least = (max_tokens + kLargest - 1) / kLargest;
+    return s < least ? 1 : (int)s;
 }
 
 size_t evict_workspace_bytes(int batch, int hkv, int max_tokens, int keep, int num_cus) {
