@@ -292,8 +292,8 @@ int validate(const fdk_decode_args* a, bool need_out, bool need_workspace_only) 
 // kv heads per workgroup of the MXFP4 kernels: two where rows of neighbouring heads are parts of the same 128-byte lines, so that
 // one compute unit reads whole lines - unless only single heads give every compute unit (evenly) a workgroup, and with it a single
 // pass, and the call is short: the combine launch then costs more than the whole lines save (batch 32 x 8 kv heads, rows of 64 bytes,
-// single heads against pairs: 10 / 17 us at 1024 tokens, 20 / 25 at 2048, 37 / 37 at 4096, 70 / 60 at 8192; rows of 32 bytes: 13 / 15
-// at 2048, 27 / 24 at 4096; batch 48, an uneven fill, 64-byte rows: 67 / 49 at 4096).
+// single heads against pairs: 11 / 17 us at 1024 tokens, 21 / 25 at 2048, 37 / 38 at 4096, 69 / 60 at 8192; rows of 32 bytes: 13 / 16
+// at 2048, 28 / 26 at 4096; batch 48, an uneven fill, 64-byte rows: 66 / 52 at 4096).
 int mx_kv_heads_per_wg(const fdk_decode_args* a, int64_t head_units, int num_cus, double stream_us) {
     const bool neighbours = a->k_stride_head == a->head_dim / 2 && a->v_stride_head == a->head_dim / 2;
     if (!neighbours || a->head_dim > 128 || a->num_kv_heads % 2) return 1;

@@ -524,7 +524,7 @@ __global__ __launch_bounds__(THREADS) void evict_move_kernel(const MoveParams m)
 
 // Segments of a row (of its capacity: the lengths are on the device): as many as give two workgroups to a compute unit, of about
 // 4096 weights or more.  One workgroup does it in one launch instead of four, up to 16384 weights out of registers; more are for
-// longer rows, and for few of them: whole calls, a quarter kept, in us, one workgroup to a row against several (rows of 256 bytes)
+// longer rows, and for few of them: whole calls in a graph, a quarter kept, in us, one workgroup to a row against several (rows of 256 bytes)
 // 8 rows of 4097 / 8192 / 16384 tokens 25 / 28 / 42 against 32 / 32 / 42, 256 rows 72 / 134 / 257 against 113 / 195 / 385; (rows of
 // 128 bytes) 8 rows of 16400 / 65536 tokens 49 / 140 against 39 / 67, 64 rows (eight segments) 78 / 258 against 79 / 190, 128 rows
 // (four) 108 / 389 against 127 / 376, 256 rows (two) 177 / 653 against 229 / 890.

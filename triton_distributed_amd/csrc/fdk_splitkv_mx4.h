@@ -20,9 +20,10 @@
 // (sequence, split) runs on one XCD, with loads that leave the lines in its L2 (tiles_on_one_xcd).  Pairs of 64-byte rows with
 // pages of 16 << n tokens go through LDS instead (fdk_splitkv_mx4_staged.hip).
 //
-// Bound by the bytes of the rows, laid out by head: 4 sequences x 8 kv heads x 131072 tokens (570 MB) in 91 us, 6.3 TB/s; 32 x 8 x 4096
-// (143 MB) in 27 us, 5.3 TB/s, fill and drain included.  The arithmetic (96 conversions and permutes, 16 MFMAs and a softmax of a step
-// of 32 tokens) is about half of that time by its instructions' rates, and runs beside the loads.
+// Bound by the bytes of the rows, laid out by head: 4 sequences x 8 kv heads x 131072 tokens (570 MB) in 97 us, 5.9 TB/s; 32 x 8 x 4096
+// (143 MB) in 27 us, 5.2 TB/s, fill and drain included; calls without the arithmetic take 87 and 24.  The arithmetic (96 conversions
+// and permutes, 16 MFMAs, a softmax and the splitting of the probabilities per step of 32 tokens) is somewhat more than half of
+// that time by its instructions' rates, and runs beside the loads.
 #pragma once
 
 #include "fdk_mxfp4.h"
@@ -493,7 +494,7 @@ __global__ __launch_bounds__(512) void splitkv_mx4_kernel(const SplitParams p, c
     // ---- pipeline ----
     // Streamed rows: two register buffers, a step's rows are requested a whole step ahead.  Rows shared through the L2: one
     // buffer, the K registers take the next step's rows as soon as the logits are there, the V registers after P V (batch 32 x
-    // 8 kv heads x 4096 tokens in a single pass: 36 us against 38 us with two).  Page numbers run a step further ahead: vector
+    // 8 kv heads x 4096 tokens in a single pass, before the probabilities had a second part: 36 us against 38 us with two).  Page numbers run a step further ahead: vector
     // loads of them in front of the rows, scalar ones behind (see fdk_splitkv_mfma_body.h).
     const int n_full = (c_end - c_start) / kStep;
     {

@@ -12,10 +12,11 @@
 // and waited for by count (loads return in order, every step issues the same number), as in fdk_splitkv_mfma_shared.h; the
 // compiler sees no other vector loads in that loop: page numbers come as scalar loads (pages of 16 << n tokens).
 //
-// Measured, 4 sequences x 8 kv heads x 131072 tokens (570 MB): 104 us, 5.5 TB/s; the loads alone take 97, pairs loaded into
-// registers (one buffer, L2) 116, eight heads per workgroup sharing four staged places behind a barrier 111.  The same rows laid
-// out by head stream at 91 (fdk_splitkv_mx4.h).  Rows of 32 bytes are not staged: four heads of a line per wavefront took 94 us
-// where pairs in registers take 70 (64 sequences x 8 kv heads x 8192 tokens).
+// Measured, whole calls, 4 sequences x 8 kv heads x 131072 tokens (570 MB): 106 us, 5.4 TB/s; without the arithmetic 98; the same
+// rows laid out by head stream at 97 (fdk_splitkv_mx4.h).  With probabilities of one part, which took 104: pairs loaded into
+// registers (one buffer, L2) 116, eight heads per workgroup sharing four staged places behind a barrier 111; and, for rows of 32
+// bytes, which are not staged, four heads of a line per wavefront 94 where pairs in registers took 70 (now 73; 64 sequences x 8
+// kv heads x 8192 tokens).
 
 #include "fdk_splitkv_mx4.h"
 

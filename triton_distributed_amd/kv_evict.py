@@ -60,7 +60,8 @@ def accumulate_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, block_t
     over the q heads ``h`` of kv head ``kvh``, for the ``kv_lens[b]`` cached tokens.
 
     q, k_cache, block_table, kv_lens, sm_scale, soft_cap, k_scale   as in ``flash_decode`` (16-bit, fp8 and MXFP4 caches)
-    lse        [B, Hq] fp32, what ``flash_decode`` returned for this query
+    lse        [B, Hq] fp32, what ``flash_decode`` returned for this query; where the tokens are spread over several ranks, the
+               merged one (``inter_rank_combine(..., all_ranks_lse=, lse_out=)``): the lse of a packed result is in 16 bits
     weights    [B, Hkv, S] fp32, updated in place; S must cover every length (tokens past S are left out)
     Returns ``weights``.  Every weight is summed in a fixed order: the same bits on every run."""
     key = (_meta(q), _meta(k_cache), _meta(block_table), _meta(kv_lens), _meta(lse), _meta(weights), _meta(k_scale), sm_scale, soft_cap)
