@@ -219,7 +219,8 @@ typedef struct fdk_decode_args {
     /* (revision 3) kv_dtype FDK_MXFP4: the scale bytes of the caches, [num_pages, P, Hkv, D/32], with byte strides of the
      * page, token and head axes; rows aligned to 4 bytes (head_dim 64: 2).  k_scale / v_scale are not read.  Built for
      * head_dim 64, 128 and 256 with v_head_dim = head_dim on the matrix-core path; no single-launch form; with counters, too, a forced split count runs as
-     * one workgroup per piece.  A value takes part as code * 2^(byte - 127) converted to q's dtype, exact within its range */
+     * one workgroup per piece.  A value takes part as code * 2^(byte - 127) converted to q's dtype, exact within its range (a
+     * cache written for bf16 and read with fp16 queries may hold values beyond 65504: infinities, and NaN where they are weighed) */
     const uint8_t* k_block_scale;
     const uint8_t* v_block_scale;
     int64_t kbs_stride_page, kbs_stride_tok, kbs_stride_head;

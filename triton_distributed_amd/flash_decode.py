@@ -554,8 +554,8 @@ def flash_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
                  equal shares of the tokens on the device (a single pass is as slow as its longest sequence) and
                  per-sequence chunks follow each sequence's own length; results never depend on it
     k_scale/v_scale  [Hkv] fp32 dequantisation scales of an fp8 cache; of an MXFP4 cache its e8m0 block scales
-                     [num_pages, P, Hkv, D/32] (uint8 or float8_e8m0fnu, value = code * 2^(byte - 127); rows aligned to
-                     4 bytes, D = 64: 2)
+                     [num_pages, P, Hkv, D/32] (uint8 or float8_e8m0fnu, value = code * 2^(byte - 127), within the range
+                     of q's dtype; rows aligned to 4 bytes, D = 64: 2)
     fp8_fold_k_scale fp8 cache: apply k_scale to the logits instead of to every K value (see ``prepare_decode``)
     force_balanced   measurement / test aid: equal shares of the whole batch whatever the planner would choose
 
